@@ -213,6 +213,47 @@ int mako_heads_clear(mako_attn_ctx* ctx, void* stream, int dtype, void* y, uint3
 int mako_proj(mako_attn_ctx* ctx, void* stream, int dtype, const void* w, const void* x, float* y, uint32_t T,
               uint32_t k, uint32_t n, uint32_t ldy);
 
+/* ---- Operators around a KV cache --------------------------------------------------------------------------------
+ * No reference counterpart: the reference keeps no cache across tokens beyond what attention() reads.  The cache is
+ * the one mako_attention_decode reads: k and v [batch][kv_heads][k_stride][dim] of `dtype`, kv_len [batch] int32 on the
+ * device, dim 64, 128 or 256; an entry of kv_len <= 0 is an empty sequence.  A step of speculative decoding appends
+ * the drafted tokens (mako_cache_append), attends them (mako_attention_tree) and keeps the accepted ones; a bounded
+ * cache decodes with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls
+ * use is never freed before the context is destroyed, so a CUDA graph that captured one stays valid when a later, larger
+ * call grows it. */
+
+/* Rotation partners: value i of the rotated part with i + rot / 2, or 2i with 2i + 1. */
+enum { MAKO_ROPE_HALVES = 1, MAKO_ROPE_PAIRS = 2 };
+/* Frequency scalings for contexts longer than those trained on. */
+enum {
+    MAKO_ROPE_PLAIN = 0,  /* f_i = theta^(-2 i / rot) */
+    MAKO_ROPE_LINEAR = 1, /* f_i / factor: positions interpolated */
+    MAKO_ROPE_BASE = 2,   /* theta * factor^(rot / (rot - 2)): the slowest pair slowed by factor, the fastest kept */
+    MAKO_ROPE_PARTS = 3   /* by parts: with r_i = context * f_i / (2 pi) turns over the trained context and
+                           * g_i = (r_i - low) / (high - low) clamped to [0, 1], f_i * (g_i + (1 - g_i) / factor) */
+};
+/* Host code, host array: the angular frequencies (radians a position) freq [rot / 2] of rotary positions with base
+ * theta over the first rot values of a head.  factor (>= 1) is read by every scaling but MAKO_ROPE_PLAIN, context
+ * (> 0), low and high (0 <= low < high) by MAKO_ROPE_PARTS.  rot is even, positive and at most 256 (above 2 for
+ * MAKO_ROPE_BASE), theta > 1. */
+int mako_rope_freqs(uint32_t rot, double theta, int scaling, double factor, double context, double low, double high,
+                    double* freq);
+
+/* Appends projected tokens to the cache.  Row b * n_tok + i of x (ld floats) is token i of sequence b: q head h at
+ * column q_col0 + h * q_stride, k and v head h at k_col0 + h * dim and v_col0 + h * dim.  For i < n_new[b] (n_new null:
+ * n_tok) each q and k head is RMS-normed times wq / wk (x / sqrt(mean(x^2) + eps) * w, fp32 [dim]; null: not normed),
+ * its first rot values (even, 0: none) are rotated as `layout` pairs them by the angle pos * freq_i and multiplied by
+ * `amplitude` (1; by-parts scaling is used with 0.1 ln(factor) + 1), and k and v go to cache row kv_len[b] + i, q to
+ * q [batch][n_tok][heads][dim].  pos [batch][n_tok] int32 (null: the cache row) differs from the row for tree drafts and
+ * after an eviction; freq [rot / 2] is double on the device, so that angles of far positions keep their accuracy.  Rows
+ * i >= n_new[b] of q are left as they are, and a k / v row that would lie at or past k_stride is dropped.  kv_len is not
+ * changed.  q, k and v 16-byte aligned, every column and stride any.  batch * n_tok below 2^31. */
+int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* x, uint32_t ld, uint32_t q_col0,
+                      uint32_t q_stride, uint32_t k_col0, uint32_t v_col0, uint32_t batch, uint32_t n_tok,
+                      const int32_t* n_new, const int32_t* kv_len, const int32_t* pos, uint32_t heads,
+                      uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
+                      const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride);
+
 /* ---- Multi-GPU: one process per GPU of one box, the peers' memory mapped through CUDA IPC ------------------------
  * No reference counterpart: mako-common drives one Apple GPU.  BASELINE's sharded forms -- heads across GPUs with the
  * outputs gathered, and one long sequence's KV cache across GPUs with a log-sum-exp combine -- are built from these.

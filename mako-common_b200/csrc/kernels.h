@@ -95,6 +95,26 @@ struct HeadsParams {
 };
 cudaError_t launch_heads(const HeadsParams& p, int dtype, cudaStream_t s);
 
+// ---- operators around a KV cache: k, v [batch][kv_heads][k_stride][dim], kv_len [batch] ------------------------------
+
+// Tokens appended to the cache: row b * n_tok + i of x is token i of sequence b (see mako_cache_append).
+struct AppendParams {
+    const float* x;
+    const int32_t* n_new;   // [batch] or null: n_tok
+    const int32_t* kv_len;  // [batch]
+    const int32_t* pos;     // [batch][n_tok] or null: the cache row
+    const double* freq;     // [rot / 2] radians a position
+    const float* wq;        // [dim] or null: not normed
+    const float* wk;
+    void* q;  // [batch][n_tok][heads][dim]
+    void* k;
+    void* v;
+    uint64_t ld;
+    uint32_t q_col0, q_stride, k_col0, v_col0, batch, n_tok, heads, kv_heads, rot, layout, k_stride, vec4;
+    float amplitude, eps;
+};
+cudaError_t launch_cache_append(const AppendParams& p, int dtype, int dim, cudaStream_t s);
+
 // ---- multi-GPU exchange (one process per GPU, peers' memory mapped through CUDA IPC) ------------------------------
 
 constexpr uint32_t kMaxRanks = 8;

@@ -6,6 +6,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -843,6 +844,89 @@ int mako_heads_clear(mako_attn_ctx* ctx, void* stream, int dtype, void* y, uint3
     if (rc == MAKO_OK)
         g_error.clear();
     return rc;
+}
+
+} // extern "C"
+
+// ---- operators around a KV cache ------------------------------------------------------------------------------------
+
+namespace {
+
+// What the cache calls share: the element type, the head layout and 16-byte aligned tensors.
+int cache_check(mako_attn_ctx* ctx, int dtype, const char* what, uint32_t heads, uint32_t kv_heads, uint32_t dim)
+{
+    if (int rc = check_ctx(ctx, dtype))
+        return rc;
+    if (dim != 64 && dim != 128 && dim != 256)
+        return fail(MAKO_EINVAL, "%s: heads of %u", what, dim);
+    if (!heads || !kv_heads || heads % kv_heads)
+        return fail(MAKO_EINVAL, "%s: %u heads over %u kv heads", what, heads, kv_heads);
+    return MAKO_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* x, uint32_t ld, uint32_t q_col0,
+                      uint32_t q_stride, uint32_t k_col0, uint32_t v_col0, uint32_t batch, uint32_t n_tok,
+                      const int32_t* n_new, const int32_t* kv_len, const int32_t* pos, uint32_t heads,
+                      uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
+                      const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride)
+{
+    if (int rc = cache_check(ctx, dtype, "cache_append", heads, kv_heads, dim))
+        return rc;
+    if (rot % 2 || rot > dim)
+        return fail(MAKO_EINVAL, "cache_append: %u rotated of a head of %u", rot, dim);
+    if (rot && ((layout != MAKO_ROPE_HALVES && layout != MAKO_ROPE_PAIRS) || !freq || !std::isfinite(amplitude)))
+        return fail(MAKO_EINVAL, "cache_append: layout %d, amplitude %g, or null freq", layout, double(amplitude));
+    if ((wq || wk) && !(eps > 0.0f && std::isfinite(eps)))
+        return fail(MAKO_EINVAL, "cache_append: eps %g with a norm weight", double(eps));
+    if (q_stride < dim || uint64_t(q_col0) + uint64_t(heads - 1) * q_stride + dim > ld ||
+        uint64_t(k_col0) + uint64_t(kv_heads) * dim > ld || uint64_t(v_col0) + uint64_t(kv_heads) * dim > ld)
+        return fail(MAKO_EINVAL, "cache_append: x rows of %u floats for q at %u (stride %u), k at %u, v at %u", ld, q_col0,
+                    q_stride, k_col0, v_col0);
+    if (!x || !kv_len || !q || !k || !v || !aligned16(q) || !aligned16(k) || !aligned16(v))
+        return fail(MAKO_EINVAL, "cache_append: null or unaligned tensor (16-byte alignment)");
+    if (uint64_t(batch) * n_tok > 0x7FFFFFFFull)
+        return fail(MAKO_EINVAL, "cache_append: %u sequences of %u tokens", batch, n_tok);
+    if (batch == 0 || n_tok == 0)
+        return MAKO_OK;
+    DeviceGuard dg(ctx->device);
+    if (dg.err != cudaSuccess)
+        return cuda_fail("set device", dg.err);
+    mako::AppendParams p{};
+    p.x = x;
+    p.n_new = n_new;
+    p.kv_len = kv_len;
+    p.pos = pos;
+    p.freq = freq;
+    p.wq = wq;
+    p.wk = wk;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.ld = ld;
+    p.q_col0 = q_col0;
+    p.q_stride = q_stride;
+    p.k_col0 = k_col0;
+    p.v_col0 = v_col0;
+    p.batch = batch;
+    p.n_tok = n_tok;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.rot = rot;
+    p.layout = uint32_t(layout);
+    p.k_stride = k_stride;
+    p.vec4 = aligned16(x) && (ld | q_col0 | q_stride | k_col0 | v_col0) % 4 == 0;
+    p.amplitude = amplitude;
+    p.eps = eps;
+    ctx->launches += 1;
+    auto st = static_cast<cudaStream_t>(stream);
+    KernelTimer t(ctx, st);
+    cudaError_t e = mako::launch_cache_append(p, dtype, int(dim), st);
+    t.stop();
+    return launched("cache_append", e);
 }
 
 } // extern "C"

@@ -14,6 +14,8 @@ LIB_PATH = os.path.join(HERE, "libmako_attn.so")
 F16, BF16 = 0, 1
 OK, EINVAL, ENOMEM, ECUDA, ENOTSUP = 0, -22, -12, -5, -95
 OPT_PREFILL_KERNEL, OPT_DECODE_ROUTE, OPT_DECODE_CHUNK, OPT_KERNEL_TIMING, OPT_OUTPUT_16BIT, OPT_GRID_CTAS = 1, 2, 3, 4, 5, 6
+ROPE_HALVES, ROPE_PAIRS = 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 UINT32_MAX = 0xFFFFFFFF
 
 # Every symbol include/mako_attn.h declares, for the load check.
@@ -24,7 +26,7 @@ SYMBOLS = (
     "mako_peer_alloc", "mako_peer_free", "mako_peer_open", "mako_peer_close", "mako_group_create", "mako_group_connect",
     "mako_group_destroy", "mako_attention_gather", "mako_attention_decode_kv_sharded", "mako_group_connect_ptrs",
     "mako_group_area", "mako_heads", "mako_heads_norm", "mako_heads_partial", "mako_heads_clear",
-    "mako_cube_layout", "mako_proj",
+    "mako_cube_layout", "mako_proj", "mako_rope_freqs", "mako_cache_append",
 )
 
 
@@ -80,6 +82,10 @@ def lib():
     L.mako_heads_clear.argtypes = [p, p, i32, p, u32, u32, u32, u32]
     L.mako_proj.argtypes = [p, p, i32, p, p, p, u32, u32, u32, u32]
     L.mako_cube_layout.argtypes = [u32] * 6 + [ctypes.c_float, p, p, p, ctypes.POINTER(CubeLayoutInfo)]
+    f64 = ctypes.c_double
+    L.mako_rope_freqs.argtypes = [u32, f64, i32, f64, f64, f64, f64, p]
+    L.mako_cache_append.argtypes = ([p, p, i32, p] + [u32] * 7 + [p, p, p] + [u32] * 4 + [i32, p, f32, p, p, f32]
+                                    + [p, p, p, u32])
     H = ctypes.POINTER(IpcHandle)
     L.mako_peer_alloc.argtypes = [p, ctypes.c_size_t, ctypes.POINTER(p), H]
     L.mako_peer_free.argtypes = [p, p]
@@ -217,6 +223,22 @@ class Context:
     def heads_clear(self, y, dim, n_pad, from_, heads, stream=None):
         _check(lib().mako_heads_clear(self._h, _stream(stream), dtype_code(y), _ptr(y), dim, n_pad, from_, heads))
 
+    # -- operators around a KV cache k, v [batch][kv_heads][k_stride][dim], kv_len int32 [batch] (no reference counterpart)
+    def cache_append(self, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new, kv_len, pos, heads, kv_heads,
+                     dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v, k_stride, stream=None):
+        """mako_cache_append: x float32 rows -> q [batch][n_tok][heads][dim] and cache rows kv_len[b] + i, normed and
+        rotated; n_new, pos, wq, wk may be None, freq a float64 tensor [rot / 2] (None when rot is 0)."""
+        _check(lib().mako_cache_append(self._h, self._stream(stream), dtype_code(q), _ptr(x), ld, q_col0, q_stride,
+                                       k_col0, v_col0, batch, n_tok, _ptr(n_new), _ptr(kv_len), _ptr(pos), heads,
+                                       kv_heads, dim, rot, layout, _ptr(freq), amplitude, _ptr(wq), _ptr(wk), eps,
+                                       _ptr(q), _ptr(k), _ptr(v), k_stride))
+
+    def _stream(self, stream):
+        """The stream given, or the current one of this context's device."""
+        import torch
+        s = torch.cuda.current_stream(self.device) if stream is None else stream
+        return ctypes.c_void_p(s.cuda_stream)
+
     # -- TransformerRuntime::cube_select (src/models/runtime.cpp:286-303); returns (sel, nsel) as int16 tensor views
     # of the context's scratch ([heads][n_cubes][min(topk, n_cubes)] and [heads][n_cubes], uint16 bit patterns),
     # valid until the next cube_select on this context.
@@ -346,3 +368,11 @@ def cube_layout(frames, ph, pw, rows_per_frame, video_row0, dense, keep):
                               map_.ctypes.data_as(ctypes.c_void_p), valid.ctypes.data_as(ctypes.c_void_p),
                               cnt.ctypes.data_as(ctypes.c_void_p), ctypes.byref(info)))
     return map_, valid, cnt[:info.n_cubes], info
+
+
+def rope_freqs(rot, theta, scaling=ROPE_PLAIN, factor=1.0, context=0.0, low=0.0, high=0.0):
+    """mako_rope_freqs: the angular frequencies of rotary positions as a numpy float64 array [rot / 2]."""
+    import numpy as np
+    freq = np.zeros(max(rot // 2, 1), np.float64)
+    _check(lib().mako_rope_freqs(rot, theta, scaling, factor, context, low, high, freq.ctypes.data_as(ctypes.c_void_p)))
+    return freq[:rot // 2]
