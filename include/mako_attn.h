@@ -254,6 +254,41 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
                       uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
                       const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride);
 
+/* Attention for a tree of drafted tokens over a cache: q [batch][n_tok][heads][dim] (n_tok at most 256), the drafted
+ * tokens' keys and values at cache rows kv_len[b] + i as mako_cache_append leaves them.  Token i < n_new[b] (null: n_tok)
+ * sees the cached keys [0, kv_len[b]) and the drafted keys j < n_new[b] with bit j % 32 of
+ * mask[b][i][j / 32] set (uint32 [batch][n_tok][(n_tok + 31) / 32]; null: j <= i, a chain); o [batch][n_tok][heads * dim]
+ * floats (or 16-bit, MAKO_OPT_OUTPUT_16BIT), rows i >= n_new[b] left as they are, a row that sees nothing is 0.
+ * A length above max_kv_len is read as max_kv_len; max_kv_len + n_tok is at most k_stride.  What cache rows hold that
+ * no token of the sequence sees, NaN or infinities among it, has no effect, and neither has a drafted token on those
+ * that do not see it. */
+int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
+                        float* o, uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len,
+                        uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t k_stride,
+                        const uint32_t* mask);
+
+/* mako_attention_decode that also accumulates every key's attention weight: weight [batch][kv_heads][k_stride] fp32
+ * receives, at key j < kv_len[b], the sum over the kv head's query heads of softmax_j added to what it held; entries at
+ * or past the length are left as they are.  The order of every sum is fixed: equal calls give equal results. */
+int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
+                                  const void* v, float* o, float* weight, uint32_t batch, const int32_t* kv_len,
+                                  uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                                  uint32_t k_stride);
+
+/* Evicts from a cache by accumulated weight.  Every sequence longer than `budget` (1 or more) keeps, for each kv head,
+ * its first `sinks` rows, its last `recent` rows (sinks + recent <= budget) and those of the rest with the largest weight
+ * until there are `budget`: equal weights keep the lower row, a NaN weight counts below all others.  The kept rows move, in
+ * their order, to rows 0, 1, ... of k_out and v_out [batch][kv_heads][out_stride][dim] and weight_out
+ * [batch][kv_heads][out_stride]; kept [batch][kv_heads][budget] int32 receives the row each came from (-1 past their
+ * number), new_len [batch] int32 min(kv_len, budget).  A sequence within the budget keeps all its rows.  Other rows of the
+ * outputs are left as they are.  In place: k_out == k, v_out == v, weight_out == weight and out_stride == k_stride;
+ * otherwise the outputs share no memory with the inputs (checked for equal addresses), except that new_len may be kv_len.
+ * budget <= out_stride; a length above max_kv_len (<= k_stride) is read as max_kv_len. */
+int mako_cache_evict(mako_attn_ctx* ctx, void* stream, int dtype, const void* k, const void* v, const float* weight,
+                     uint32_t batch, const int32_t* kv_len, uint32_t max_kv_len, uint32_t kv_heads, uint32_t dim,
+                     uint32_t k_stride, uint32_t sinks, uint32_t recent, uint32_t budget, void* k_out, void* v_out,
+                     float* weight_out, uint32_t out_stride, int32_t* kept, int32_t* new_len);
+
 /* ---- Multi-GPU: one process per GPU of one box, the peers' memory mapped through CUDA IPC ------------------------
  * No reference counterpart: mako-common drives one Apple GPU.  BASELINE's sharded forms -- heads across GPUs with the
  * outputs gathered, and one long sequence's KV cache across GPUs with a log-sum-exp combine -- are built from these.

@@ -9,6 +9,10 @@
 // mma.sync (the group's q rows padded to 16), keeps its own running softmax and accumulator, and the warps merge at
 // the end into one partial (o unnormalised, max, sum) per (sequence, head, split); a sequence with one split writes
 // o directly.
+// The same kernel serves two more calls: with SCORES it also stores every scaled score, from which
+// decode_weights_kernel makes the keys' attention weights once the row's maximum and sum are known; with TREE the rows
+// of a kv head are the drafted tokens times the group's heads, and the drafted keys behind the cached ones are seen by
+// mask.
 // Kernel 2 (decode_combine_kernel): the log-sum-exp merge of a row's splits into o, launched as a programmatic
 // dependent of kernel 1 so that its launch overlaps kernel 1's last wave.
 #include "common.cuh"
@@ -24,6 +28,8 @@ namespace {
 constexpr int DBN = 64, DNT = 128, DST = 3, QR = 16;
 constexpr uint64_t kMaxSplits = 1024;
 
+enum Mode { PLAIN, SCORES, TREE };
+
 // Keys of sequence b: its kv_len entry (<= 0: none) capped at max_kv_len, so that a length beyond the split plan's
 // reach is cut at max_kv_len and every kernel of a call agrees on the same split count; without kv_len, p.len.
 __device__ __forceinline__ uint32_t seq_keys(const DecodeParams& p, uint32_t b)
@@ -34,7 +40,30 @@ __device__ __forceinline__ uint32_t seq_keys(const DecodeParams& p, uint32_t b)
     return l > 0 ? min(uint32_t(l), p.len) : 0u;
 }
 
-template <int D, typename T>
+// Drafted tokens of sequence b (TREE).
+__device__ __forceinline__ uint32_t seq_new(const DecodeParams& p, uint32_t b)
+{
+    if (!p.n_new)
+        return p.n_tok;
+    const int32_t n = p.n_new[b];
+    return n > 0 ? min(uint32_t(n), p.n_tok) : 0u;
+}
+// Whether token tok of sequence b sees drafted token j (TREE).
+__device__ __forceinline__ bool tree_sees(const DecodeParams& p, uint32_t b, uint32_t tok, uint32_t j)
+{
+    if (!p.mask)
+        return j <= tok;
+    return __ldg(p.mask + (uint64_t(b) * p.n_tok + tok) * ((p.n_tok + 31) / 32) + j / 32) >> (j % 32) & 1u;
+}
+
+// A row's value: 0 for a row that sees no key; a NaN sum stays NaN (MODE != PLAIN).
+template <int MODE>
+__device__ __forceinline__ float row_value(float o, float l)
+{
+    return (MODE == PLAIN ? l > 0.0f : l != 0.0f) ? o / l : 0.0f;
+}
+
+template <int D, typename T, int MODE>
 __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams p)
 {
     constexpr int ROWB = D * 2, CH = D / 8, KS = D / 16, TILE = DBN * ROWB;
@@ -42,16 +71,29 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t sQ = smem_u32(smem), sK = sQ + QR * ROWB, sV = sK + DST * TILE;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3, mi = lane >> 3;
-    const uint32_t group = p.heads / p.kv_heads, rb = (group + QR - 1) / QR;
+    const uint32_t group = p.heads / p.kv_heads, rows = MODE == TREE ? group * p.n_tok : group, rb = (rows + QR - 1) / QR;
     const uint32_t b = blockIdx.z, kvh = blockIdx.y / rb, rblk = blockIdx.y % rb, split = blockIdx.x;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the combine may be scheduled now
-    const uint32_t L = seq_keys(p, b);
+    const uint32_t cached = seq_keys(p, b), drafted = MODE == TREE ? seq_new(p, b) : 0u, L = cached + drafted;
     const uint32_t start = split * p.chunk;
-    const uint32_t h0 = kvh * group + rblk * QR, nrows = min(uint32_t(QR), group - rblk * QR);
+    const uint32_t live = MODE == TREE ? group * drafted : group;
+    if (MODE == TREE && rblk * QR >= live)
+        return;
+    const uint32_t h0 = kvh * group + rblk * QR, nrows = min(uint32_t(QR), live - rblk * QR);
+    // the (token, head) of row r as an index into q's and o's rows
+    auto row_head = [&](uint32_t r) {
+        if (MODE != TREE)
+            return h0 + r;
+        const uint32_t t = rblk * QR + r;
+        return t / group * p.heads + kvh * group + t % group;
+    };
+    __shared__ uint32_t bad[8];  // TREE: drafted tokens of this split whose values are not all finite
+    if (MODE == TREE && tid < 8)
+        bad[tid] = 0;
     if (start >= L) {
         if (L == 0 && split == 0 && !p.keep_partials)  // no key: the rows are 0
             for (uint32_t i = tid; i < nrows * D; i += DNT)
-                out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + i / D) * D + i % D, 0.0f, p.o_type);
+                out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(row_head(i / D)) * D + i % D, 0.0f, p.o_type);
         return;
     }
     const uint32_t end = min(L, start + p.chunk);
@@ -62,7 +104,7 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
     for (int i = tid; i < QR * CH; i += DNT) {
         const uint32_t r = i / CH, c = i % CH;
         const bool ok = r < nrows;
-        cp_async16(sQ + swz(r, c, ROWB), qg + (ok ? uint64_t(h0 + r) * p.q_hstride + c * 8 : 0), ok);
+        cp_async16(sQ + swz(r, c, ROWB), qg + (ok ? uint64_t(row_head(r)) * p.q_hstride + c * 8 : 0), ok);
     }
     cp_async_commit();
     const uint32_t nt = (end - start + DBN - 1) / DBN;
@@ -104,6 +146,21 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
         cp_async_commit();
         const uint32_t kst = sK + (t % DST) * TILE, vst = sV + (t % DST) * TILE;
         const uint32_t kr = warp * 16;  // this warp's 16 keys of the tile
+        if (MODE == TREE && start + t * DBN + DBN > cached) {
+            // Drafted keys: a value that is not finite becomes 0 here, so that P = 0 drops it from the rows that do not
+            // see its token; the rows that do add it back at the end.
+            for (int i = tid; i < DBN * D; i += DNT) {
+                const uint32_t r = i / D, d = i % D, j = start + t * DBN + r;
+                if (j >= cached && j < end) {
+                    T* const e = reinterpret_cast<T*>(smem + QR * ROWB + DST * TILE + (t % DST) * TILE + swz(r, d / 8, ROWB)) + d % 8;
+                    if (!isfinite(Elem<T>::to_f(*e))) {
+                        *e = T(0.0f);
+                        atomicOr(&bad[(j - cached) / 32], 1u << ((j - cached) % 32));
+                    }
+                }
+            }
+            __syncthreads();
+        }
 
         float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -120,10 +177,23 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t j = jb + n * 8 + 2 * tq + (e & 1);
-                const float x = j < end ? s[n][e] * scale : -INFINITY;
+                bool see = j < end;
+                if (MODE == TREE && see && j >= cached)
+                    see = tree_sees(p, b, min((rblk * QR + g + 8 * (e >> 1)) / group, p.n_tok - 1), j - cached);
+                const float x = see ? s[n][e] * scale : -INFINITY;
                 s[n][e] = x;
                 mx[e >> 1] = fmaxf(mx[e >> 1], x);
             }
+        if (MODE == SCORES) {
+            // rows of s_stride (a multiple of 64) scores, so that a tile's last pair lies within its row
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (uint32_t(g + 8 * r) < nrows)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+                        *reinterpret_cast<float2*>(p.scores + (uint64_t(b) * p.heads + h0 + g + 8 * r) * p.s_stride + jb +
+                                                   n * 8 + 2 * tq) = make_float2(s[n][2 * r], s[n][2 * r + 1]);
+        }
         float f[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -146,7 +216,8 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float mm = m[e >> 1];
-                const float pe = mm == -INFINITY ? 0.0f : ex2(s[n][e] - mm);
+                // (MODE != PLAIN) a NaN score of a row with no maximum yet still makes its sum NaN
+                const float pe = mm == -INFINITY ? (MODE != PLAIN && s[n][e] != s[n][e] ? s[n][e] : 0.0f) : ex2(s[n][e] - mm);
                 s[n][e] = pe;
                 l[e >> 1] += pe;
             }
@@ -212,10 +283,22 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
             Ls += sm[(w * 2 + 1) * QR + r] * fw;
             O += so[(w * QR + r) * D + d] * fw;
         }
+        if (MODE == TREE) {
+#pragma unroll 1
+            for (int w = 0; w < 8; ++w)
+                for (uint32_t m = bad[w]; m; m &= m - 1) {
+                    const uint32_t j = w * 32 + __ffs(m) - 1;
+                    const float x = Elem<T>::to_f(vg[uint64_t(cached + j) * D + d]);
+                    if (!isfinite(x) && tree_sees(p, b, (rblk * QR + r) / group, j))
+                        O += x;
+                }
+        }
+        if (MODE == SCORES && d == 0 && ns == 1)
+            p.ml_part[(uint64_t(b) * p.heads + h0 + r) * p.n_splits] = make_float2(M, Ls);
         if (ns == 1 && !p.keep_partials) {
-            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + r) * D + d, Ls > 0.0f ? O / Ls : 0.0f, p.o_type);
+            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(row_head(r)) * D + d, row_value<MODE>(O, Ls), p.o_type);
         } else {
-            const uint64_t row = (uint64_t(b) * p.heads + h0 + r) * p.n_splits + split;
+            const uint64_t row = (uint64_t(b) * (MODE == TREE ? p.n_tok * p.heads : p.heads) + row_head(r)) * p.n_splits + split;
             p.o_part[row * D + d] = O;
             if (d == 0)
                 p.ml_part[row] = make_float2(M, Ls);
@@ -225,18 +308,20 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 
 // One CTA per (head, sequence), one thread per output value; the splits' weights 2^(m_s - M) go through shared
 // memory so each thread's loop is a stream of independent loads.
-template <int D>
+template <int D, int MODE>
 __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
 {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");  // kernel 1's writes are visible from here on
     __shared__ float w[kMaxSplits];
     __shared__ float tot;
-    const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-    const uint32_t L = seq_keys(p, b);
+    const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;  // TREE: h = token * heads + head
+    const uint32_t L = seq_keys(p, b) + (MODE == TREE ? seq_new(p, b) : 0u);
     const uint32_t ns = min((L + p.chunk - 1) / p.chunk, p.n_splits);
     if (ns <= 1)  // written by kernel 1 (one split, or no key)
         return;
-    const uint64_t row0 = (uint64_t(b) * p.heads + h) * p.n_splits;
+    if (MODE == TREE && h / p.heads >= seq_new(p, b))
+        return;
+    const uint64_t row0 = (uint64_t(b) * gridDim.x + h) * p.n_splits;
     float M = -INFINITY;
     for (uint32_t s = d; s < ns; s += D)
         M = fmaxf(M, p.ml_part[row0 + s].x);
@@ -284,7 +369,61 @@ __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
     for (; s < ns; ++s)
         acc[0] += src[uint64_t(s) * D] * w[s];
     const float O = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
-    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, tot > 0.0f ? O / tot : 0.0f, p.o_type);
+    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, row_value<MODE>(O, tot), p.o_type);
+}
+
+// The keys' attention weights from the stored scores (SCORES): a CTA takes WKEYS keys of one kv head.  First a warp a
+// head merges the head's splits into its maximum and sum; then each thread sums 2^(s - max) / sum over the group's heads
+// for four keys, in the heads' order, and adds that to their weights.  Reads 4 bytes a (key, head), reads and writes 4 a
+// key.
+constexpr uint32_t WNT = 256, WKEYS = 4 * WNT, WHEADS = 64;
+__global__ void __launch_bounds__(WNT) decode_weights_kernel(const DecodeParams p)
+{
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    __shared__ float2 ml[WHEADS];  // (max, 1 / sum) of up to WHEADS heads at a time
+    const uint32_t b = blockIdx.z, kvh = blockIdx.y, group = p.heads / p.kv_heads;
+    const uint32_t L = seq_keys(p, b), j = blockIdx.x * WKEYS + threadIdx.x * 4;
+    if (blockIdx.x * WKEYS >= L)
+        return;
+    const uint32_t ns = min((L + p.chunk - 1) / p.chunk, p.n_splits);
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t h0 = 0; h0 < group; h0 += WHEADS) {
+        const uint32_t nh = min(WHEADS, group - h0);
+        __syncthreads();
+        for (uint32_t h = threadIdx.x / 32; h < nh; h += WNT / 32) {
+            const float2* src = p.ml_part + (uint64_t(b) * p.heads + kvh * group + h0 + h) * p.n_splits;
+            float M = -INFINITY, l = 0.0f;
+            for (uint32_t s = threadIdx.x % 32; s < ns; s += 32)
+                M = fmaxf(M, src[s].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            for (uint32_t s = threadIdx.x % 32; s < ns; s += 32)
+                l += src[s].x == -INFINITY ? 0.0f : src[s].y * ex2(src[s].x - M);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (threadIdx.x % 32 == 0)
+                ml[h] = M == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / l);
+        }
+        __syncthreads();
+        if (j < L) {
+            const float* s = p.scores + (uint64_t(b) * p.heads + kvh * group + h0) * p.s_stride + j;
+            for (uint32_t h = 0; h < nh; ++h, s += p.s_stride) {
+                const float4 x = *reinterpret_cast<const float4*>(s);
+                const float2 c = ml[h];
+                acc[0] += ex2(x.x - c.x) * c.y;
+                acc[1] += ex2(x.y - c.x) * c.y;
+                acc[2] += ex2(x.z - c.x) * c.y;
+                acc[3] += ex2(x.w - c.x) * c.y;
+            }
+        }
+    }
+    float* w = p.weight + (uint64_t(b) * p.kv_heads + kvh) * p.w_stride + j;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < L)
+            w[e] += acc[e];
 }
 
 template <int D, typename T>
@@ -292,7 +431,7 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
     static_assert((4 * 2 * QR + 4 * QR * D) * 4 <= 2 * DST * DBN * D * 2, "merge buffer fits the stage ring");
-    auto kern = decode_split_kernel<D, T>;
+    auto kern = decode_split_kernel<D, T, PLAIN>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
@@ -309,18 +448,18 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D>, p);
+    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, PLAIN>, p);
 }
 
-template <int D, typename T>
+template <int D, typename T, int MODE>
 cudaError_t launch_split_only(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
-    auto kern = decode_split_kernel<D, T>;
+    auto kern = decode_split_kernel<D, T, MODE>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
-    const uint32_t group = p.heads / p.kv_heads, rb = (group + QR - 1) / QR;
+    const uint32_t rows = p.heads / p.kv_heads * (MODE == TREE ? p.n_tok : 1u), rb = (rows + QR - 1) / QR;
     kern<<<dim3(p.n_splits, p.kv_heads * rb, p.batch), DNT, smem, st>>>(p);
     return cudaGetLastError();
 }
@@ -473,11 +612,11 @@ cudaError_t launch_decode_split(const DecodeParams& p, int dtype, int dim, cudaS
     const bool bf = dtype == kBF16;
     switch (dim) {
     case 64:
-        return bf ? launch_split_only<64, __nv_bfloat16>(p, st) : launch_split_only<64, __half>(p, st);
+        return bf ? launch_split_only<64, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<64, __half, PLAIN>(p, st);
     case 128:
-        return bf ? launch_split_only<128, __nv_bfloat16>(p, st) : launch_split_only<128, __half>(p, st);
+        return bf ? launch_split_only<128, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<128, __half, PLAIN>(p, st);
     case 256:
-        return bf ? launch_split_only<256, __nv_bfloat16>(p, st) : launch_split_only<256, __half>(p, st);
+        return bf ? launch_split_only<256, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<256, __half, PLAIN>(p, st);
     default:
         return cudaErrorInvalidValue;
     }
@@ -498,14 +637,71 @@ cudaError_t launch_decode_combine(const DecodeParams& p, int dim, cudaStream_t s
     cfg.numAttrs = 1;
     switch (dim) {
     case 64:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64, PLAIN>, p);
     case 128:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128, PLAIN>, p);
     case 256:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256, PLAIN>, p);
     default:
         return cudaErrorInvalidValue;
     }
+}
+
+namespace {
+
+// A programmatic dependent of the stream's last kernel.
+cudaLaunchConfig_t dependent(dim3 grid, dim3 block, cudaStream_t st, cudaLaunchAttribute* attr)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+template <int D>
+cudaError_t launch_tree_d(const DecodeParams& p, bool bf, cudaStream_t st)
+{
+    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, TREE>(p, st) : launch_split_only<D, __half, TREE>(p, st);
+    if (e != cudaSuccess)
+        return e;
+    cudaLaunchAttribute attr;
+    const auto cfg = dependent(dim3(p.heads * p.n_tok, p.batch), dim3(D), st, &attr);
+    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, TREE>, p);
+}
+
+template <int D>
+cudaError_t launch_weights_d(const DecodeParams& p, bool bf, cudaStream_t st)
+{
+    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, SCORES>(p, st) : launch_split_only<D, __half, SCORES>(p, st);
+    if (e != cudaSuccess)
+        return e;
+    cudaLaunchAttribute attr;
+    auto cfg = dependent(dim3(p.heads, p.batch), dim3(D), st, &attr);
+    if ((e = cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, SCORES>, p)) != cudaSuccess || p.len == 0)
+        return e;
+    cfg = dependent(dim3((p.len + WKEYS - 1) / WKEYS, p.kv_heads, p.batch), dim3(WNT), st, &attr);
+    return cudaLaunchKernelEx(&cfg, decode_weights_kernel, p);
+}
+
+} // namespace
+
+cudaError_t launch_tree(const DecodeParams& p, int dtype, int dim, cudaStream_t st)
+{
+    const bool bf = dtype == kBF16;
+    return dim == 64 ? launch_tree_d<64>(p, bf, st) : dim == 128 ? launch_tree_d<128>(p, bf, st) : launch_tree_d<256>(p, bf, st);
+}
+
+cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t st)
+{
+    const bool bf = dtype == kBF16;
+    return dim == 64    ? launch_weights_d<64>(p, bf, st)
+           : dim == 128 ? launch_weights_d<128>(p, bf, st)
+                        : launch_weights_d<256>(p, bf, st);
 }
 
 cudaError_t launch_decode_xchg(const DecodeParams& p, const XchgParams& x, int dim, cudaStream_t st)

@@ -73,12 +73,26 @@ struct DecodeParams {
     float scale;
     uint32_t keep_partials;  // 1: always write partials (the KV-sharded combine reads them), never o
     uint32_t o_type;         // element type of o: 0 fp32, 1 fp16, 2 bf16
+    // decode with weights: scores [batch][heads][s_stride] (scaled, log2 units), weight [batch][kv_heads][w_stride]
+    float* scores;
+    float* weight;
+    uint64_t s_stride, w_stride;
+    // tree: rows are (token, head) pairs, q and o [batch][n_tok][heads][dim]; kv_len counts the cached keys, the
+    // drafted ones follow; o_part and ml_part have n_tok * heads rows a sequence
+    const int32_t* n_new;  // [batch] or null: n_tok
+    const uint32_t* mask;  // [batch][n_tok][(n_tok + 31) / 32] or null: a chain
+    uint32_t n_tok;
 };
 // Keys a split takes and how many splits, for the longest sequence max_len (chunk_opt: 0 automatic, else the
 // requested multiple of 64).
 void decode_plan(uint32_t max_len, uint32_t batch, uint32_t kv_heads, uint32_t heads, int num_sms, uint32_t chunk_opt,
                  uint32_t* chunk, uint32_t* n_splits);
 cudaError_t launch_decode(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
+
+// Tree attention: the splits over cached and drafted keys, then the combine.
+cudaError_t launch_tree(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
+// Decode that also adds every key's attention weight to p.weight: splits, combine, weights.
+cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
 
 // Head-tile producers: y [heads][n_pad][dim] 16-bit, row row0 + r from x row map[r] (or r): head h's values at
 // x + row * ld + col0 + h * stride, RMS-normed times w when eps > 0, rotated when rope is 1 (halves i, i + rot / 2 over
@@ -113,6 +127,21 @@ struct AppendParams {
     uint32_t q_col0, q_stride, k_col0, v_col0, batch, n_tok, heads, kv_heads, rot, layout, k_stride, vec4;
     float amplitude, eps;
 };
+// Eviction by weight (see mako_cache_evict).
+struct EvictParams {
+    const void* k;
+    const void* v;
+    const float* weight;
+    const int32_t* kv_len;
+    void* k_out;
+    void* v_out;
+    float* weight_out;
+    int32_t* kept;     // [batch][kv_heads][budget]
+    int32_t* new_len;  // [batch], may be kv_len
+    int32_t* count;    // scratch [batch]: the rows each sequence keeps
+    uint32_t batch, max_len, kv_heads, dim, k_stride, out_stride, sinks, recent, budget, in_place;
+};
+cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s);
 cudaError_t launch_cache_append(const AppendParams& p, int dtype, int dim, cudaStream_t s);
 
 // ---- multi-GPU exchange (one process per GPU, peers' memory mapped through CUDA IPC) ------------------------------

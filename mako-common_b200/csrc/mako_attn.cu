@@ -6,6 +6,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -37,6 +38,7 @@ struct mako_attn_ctx {
         size_t bytes = 0;
     };
     std::unordered_map<std::string, Buf> scratch;
+    std::vector<void*> retired;  // outgrown buffers of scratch_kept, freed with the context
 };
 
 namespace {
@@ -113,6 +115,37 @@ int scratch(mako_attn_ctx* ctx, const char* name, size_t bytes, void** out)
     }
     *out = b.ptr;
     return MAKO_OK;
+}
+
+// As scratch, but an outgrown buffer lives on until the context is destroyed: a CUDA graph that captured a call with it
+// may still be replayed.  A buffer at least doubles when it grows, so the retired ones together stay below the last.
+int scratch_kept(mako_attn_ctx* ctx, const char* name, size_t bytes, void** out)
+try {
+    auto& b = ctx->scratch[name];
+    if (b.bytes < bytes) {
+        ctx->retired.reserve(ctx->retired.size() + 1);
+        const size_t want = std::max(bytes, 2 * b.bytes);
+        void* ptr = nullptr;
+        size_t got = want;
+        cudaError_t e = cudaMalloc(&ptr, want);
+        if (e == cudaErrorMemoryAllocation && want > bytes) {
+            cudaGetLastError();
+            got = bytes;
+            e = cudaMalloc(&ptr, bytes);
+        }
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(MAKO_ENOMEM, "scratch %s: %zu bytes: %s", name, bytes, cudaGetErrorString(e));
+        }
+        if (b.ptr)
+            ctx->retired.push_back(b.ptr);
+        b.ptr = ptr;
+        b.bytes = got;
+    }
+    *out = b.ptr;
+    return MAKO_OK;
+} catch (const std::bad_alloc&) {
+    return fail(MAKO_ENOMEM, "scratch %s", name);
 }
 
 int check_ctx(mako_attn_ctx* ctx, int dtype)
@@ -223,6 +256,8 @@ int mako_attn_destroy(mako_attn_ctx* ctx)
                 if (e != cudaSuccess && rc == MAKO_OK)
                     rc = cuda_fail("scratch free", e);
             }
+        for (void* ptr : ctx->retired)
+            cudaFree(ptr);
     }
     delete ctx;
     return rc;
@@ -886,12 +921,12 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
         uint64_t(k_col0) + uint64_t(kv_heads) * dim > ld || uint64_t(v_col0) + uint64_t(kv_heads) * dim > ld)
         return fail(MAKO_EINVAL, "cache_append: x rows of %u floats for q at %u (stride %u), k at %u, v at %u", ld, q_col0,
                     q_stride, k_col0, v_col0);
+    if (batch == 0 || n_tok == 0)
+        return MAKO_OK;
     if (!x || !kv_len || !q || !k || !v || !aligned16(q) || !aligned16(k) || !aligned16(v))
         return fail(MAKO_EINVAL, "cache_append: null or unaligned tensor (16-byte alignment)");
     if (uint64_t(batch) * n_tok > 0x7FFFFFFFull)
         return fail(MAKO_EINVAL, "cache_append: %u sequences of %u tokens", batch, n_tok);
-    if (batch == 0 || n_tok == 0)
-        return MAKO_OK;
     DeviceGuard dg(ctx->device);
     if (dg.err != cudaSuccess)
         return cuda_fail("set device", dg.err);
@@ -927,6 +962,179 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
     cudaError_t e = mako::launch_cache_append(p, dtype, int(dim), st);
     t.stop();
     return launched("cache_append", e);
+}
+
+int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
+                        float* o, uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len,
+                        uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t k_stride,
+                        const uint32_t* mask)
+{
+    if (int rc = cache_check(ctx, dtype, "tree", heads, kv_heads, dim))
+        return rc;
+    if (n_tok > 256)
+        return fail(MAKO_EINVAL, "tree: %u drafted tokens (at most 256)", n_tok);
+    if (uint64_t(max_kv_len) + n_tok > k_stride)
+        return fail(MAKO_EINVAL, "tree: max_kv_len %u and %u drafted beyond the cache's %u rows", max_kv_len, n_tok,
+                    k_stride);
+    if (batch > 65535 || uint64_t(n_tok) * heads > 65535)
+        return fail(MAKO_EINVAL, "tree: %u sequences of %u tokens, %u heads", batch, n_tok, heads);
+    if (batch == 0 || n_tok == 0)
+        return MAKO_OK;
+    if (!q || !k || !v || !o || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
+        return fail(MAKO_EINVAL, "tree: null or unaligned tensor (16-byte alignment)");
+    DeviceGuard dg(ctx->device);
+    if (dg.err != cudaSuccess)
+        return cuda_fail("set device", dg.err);
+    mako::DecodeParams p{};
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.o = o;
+    p.kv_len = kv_len;
+    p.len = max_kv_len;
+    p.q_bstride = uint64_t(n_tok) * heads * dim;
+    p.q_hstride = dim;
+    p.k_hstride = uint64_t(k_stride) * dim;
+    p.k_bstride = uint64_t(kv_heads) * p.k_hstride;
+    p.o_bstride = p.q_bstride;
+    p.o_type = out_type(ctx, dtype);
+    p.batch = batch;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.scale = 1.0f / sqrtf(float(dim));
+    p.n_new = n_new;
+    p.mask = mask;
+    p.n_tok = n_tok;
+    mako::decode_plan(max_kv_len + n_tok, batch, kv_heads, heads, ctx->num_sms, 0, &p.chunk, &p.n_splits);
+    const size_t rows = size_t(batch) * n_tok * heads * p.n_splits;
+    void *op, *mlp;
+    if (int rc = scratch_kept(ctx, "tree_o", rows * dim * 4, &op))
+        return rc;
+    if (int rc = scratch_kept(ctx, "tree_ml", rows * 8, &mlp))
+        return rc;
+    p.o_part = static_cast<float*>(op);
+    p.ml_part = static_cast<float2*>(mlp);
+    ctx->launches += 2;
+    auto st = static_cast<cudaStream_t>(stream);
+    KernelTimer t(ctx, st);
+    cudaError_t e = mako::launch_tree(p, dtype, int(dim), st);
+    t.stop();
+    return launched("tree", e);
+}
+
+int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
+                                  const void* v, float* o, float* weight, uint32_t batch, const int32_t* kv_len,
+                                  uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                                  uint32_t k_stride)
+{
+    if (int rc = cache_check(ctx, dtype, "decode_weights", heads, kv_heads, dim))
+        return rc;
+    if (max_kv_len > k_stride)
+        return fail(MAKO_EINVAL, "decode_weights: max_kv_len %u beyond the cache's %u rows", max_kv_len, k_stride);
+    if (batch > 65535 || heads > 65535)
+        return fail(MAKO_EINVAL, "decode_weights: %u sequences, %u heads", batch, heads);
+    if (batch == 0)
+        return MAKO_OK;
+    if (!q || !k || !v || !o || !weight || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
+        return fail(MAKO_EINVAL, "decode_weights: null or unaligned tensor (16-byte alignment)");
+    DeviceGuard dg(ctx->device);
+    if (dg.err != cudaSuccess)
+        return cuda_fail("set device", dg.err);
+    mako::DecodeParams p{};
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.o = o;
+    p.kv_len = kv_len;
+    p.len = max_kv_len;
+    p.q_bstride = uint64_t(heads) * dim;
+    p.q_hstride = dim;
+    p.k_hstride = uint64_t(k_stride) * dim;
+    p.k_bstride = uint64_t(kv_heads) * p.k_hstride;
+    p.o_bstride = uint64_t(heads) * dim;
+    p.o_type = out_type(ctx, dtype);
+    p.batch = batch;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.scale = 1.0f / sqrtf(float(dim));
+    mako::decode_plan(max_kv_len, batch, kv_heads, heads, ctx->num_sms, ctx->decode_chunk, &p.chunk, &p.n_splits);
+    p.weight = weight;
+    p.w_stride = k_stride;
+    p.s_stride = (uint64_t(max_kv_len) + 63) / 64 * 64;
+    void *op, *mlp, *sc;
+    if (int rc = scratch_kept(ctx, "dw_o", size_t(batch) * heads * p.n_splits * dim * 4, &op))
+        return rc;
+    if (int rc = scratch_kept(ctx, "dw_ml", size_t(batch) * heads * p.n_splits * 8, &mlp))
+        return rc;
+    if (int rc = scratch_kept(ctx, "dw_scores", size_t(batch) * heads * p.s_stride * 4, &sc))
+        return rc;
+    p.o_part = static_cast<float*>(op);
+    p.ml_part = static_cast<float2*>(mlp);
+    p.scores = static_cast<float*>(sc);
+    ctx->launches += 3;
+    auto st = static_cast<cudaStream_t>(stream);
+    KernelTimer t(ctx, st);
+    cudaError_t e = mako::launch_decode_weights(p, dtype, int(dim), st);
+    t.stop();
+    return launched("decode_weights", e);
+}
+
+int mako_cache_evict(mako_attn_ctx* ctx, void* stream, int dtype, const void* k, const void* v, const float* weight,
+                     uint32_t batch, const int32_t* kv_len, uint32_t max_kv_len, uint32_t kv_heads, uint32_t dim,
+                     uint32_t k_stride, uint32_t sinks, uint32_t recent, uint32_t budget, void* k_out, void* v_out,
+                     float* weight_out, uint32_t out_stride, int32_t* kept, int32_t* new_len)
+{
+    if (int rc = cache_check(ctx, dtype, "cache_evict", kv_heads, kv_heads, dim))
+        return rc;
+    if (!budget || uint64_t(sinks) + recent > budget || budget > out_stride || budget > 0x7FFFFFFFu)
+        return fail(MAKO_EINVAL, "cache_evict: budget %u for %u sinks and %u recent, %u output rows", budget, sinks,
+                    recent, out_stride);
+    if (max_kv_len > k_stride || max_kv_len > 0x7FFFFFFFu)
+        return fail(MAKO_EINVAL, "cache_evict: max_kv_len %u beyond the cache's %u rows", max_kv_len, k_stride);
+    if (batch > 65535 || kv_heads > 65535)
+        return fail(MAKO_EINVAL, "cache_evict: %u sequences, %u kv heads", batch, kv_heads);
+    if (batch == 0)
+        return MAKO_OK;
+    if (!k || !v || !weight || !kv_len || !k_out || !v_out || !weight_out || !kept || !new_len || !aligned16(k) ||
+        !aligned16(v) || !aligned16(k_out) || !aligned16(v_out))
+        return fail(MAKO_EINVAL, "cache_evict: null or unaligned tensor (16-byte alignment)");
+    const int same = int(k_out == k) + int(v_out == v) + int(weight_out == weight);
+    if ((same && same != 3) || (same == 3 && out_stride != k_stride) || k_out == v_out || k_out == v || v_out == k)
+        return fail(MAKO_EINVAL, "cache_evict: outputs that are partly the inputs (in place: all three, out_stride = "
+                                 "k_stride)");
+    DeviceGuard dg(ctx->device);
+    if (dg.err != cudaSuccess)
+        return cuda_fail("set device", dg.err);
+    void* count;
+    if (int rc = scratch_kept(ctx, "evict_count", size_t(batch) * 4, &count))
+        return rc;
+    mako::EvictParams p{};
+    p.k = k;
+    p.v = v;
+    p.weight = weight;
+    p.kv_len = kv_len;
+    p.k_out = k_out;
+    p.v_out = v_out;
+    p.weight_out = weight_out;
+    p.kept = kept;
+    p.new_len = new_len;
+    p.count = static_cast<int32_t*>(count);
+    p.batch = batch;
+    p.max_len = max_kv_len;
+    p.kv_heads = kv_heads;
+    p.dim = dim;
+    p.k_stride = k_stride;
+    p.out_stride = out_stride;
+    p.sinks = sinks;
+    p.recent = recent;
+    p.budget = budget;
+    p.in_place = same == 3;
+    ctx->launches += 2;
+    auto st = static_cast<cudaStream_t>(stream);
+    KernelTimer t(ctx, st);
+    cudaError_t e = mako::launch_cache_evict(p, st);
+    t.stop();
+    return launched("cache_evict", e);
 }
 
 } // extern "C"

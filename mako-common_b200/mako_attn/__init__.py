@@ -27,6 +27,7 @@ SYMBOLS = (
     "mako_group_destroy", "mako_attention_gather", "mako_attention_decode_kv_sharded", "mako_group_connect_ptrs",
     "mako_group_area", "mako_heads", "mako_heads_norm", "mako_heads_partial", "mako_heads_clear",
     "mako_cube_layout", "mako_proj", "mako_rope_freqs", "mako_cache_append",
+    "mako_attention_tree", "mako_attention_decode_weights", "mako_cache_evict",
 )
 
 
@@ -86,6 +87,9 @@ def lib():
     L.mako_rope_freqs.argtypes = [u32, f64, i32, f64, f64, f64, f64, p]
     L.mako_cache_append.argtypes = ([p, p, i32, p] + [u32] * 7 + [p, p, p] + [u32] * 4 + [i32, p, f32, p, p, f32]
                                     + [p, p, p, u32])
+    L.mako_attention_tree.argtypes = [p, p, i32, p, p, p, p, u32, u32, p, p] + [u32] * 5 + [p]
+    L.mako_attention_decode_weights.argtypes = [p, p, i32, p, p, p, p, p, u32, p] + [u32] * 5
+    L.mako_cache_evict.argtypes = [p, p, i32, p, p, p, u32, p] + [u32] * 7 + [p, p, p, u32, p, p]
     H = ctypes.POINTER(IpcHandle)
     L.mako_peer_alloc.argtypes = [p, ctypes.c_size_t, ctypes.POINTER(p), H]
     L.mako_peer_free.argtypes = [p, p]
@@ -232,6 +236,29 @@ class Context:
                                        k_col0, v_col0, batch, n_tok, _ptr(n_new), _ptr(kv_len), _ptr(pos), heads,
                                        kv_heads, dim, rot, layout, _ptr(freq), amplitude, _ptr(wq), _ptr(wk), eps,
                                        _ptr(q), _ptr(k), _ptr(v), k_stride))
+
+    def attention_tree(self, q, k, v, o, batch, n_tok, n_new, kv_len, max_kv_len, heads, kv_heads, dim, k_stride,
+                       mask=None, stream=None):
+        """mako_attention_tree: q [batch][n_tok][heads][dim] over the cache and the n_new[b] (None: n_tok) drafted rows
+        behind kv_len[b]; mask int32 or uint32 words [batch][n_tok][ceil(n_tok / 32)], None: a chain."""
+        _check(lib().mako_attention_tree(self._h, self._stream(stream), dtype_code(q), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
+                                         batch, n_tok, _ptr(n_new), _ptr(kv_len), max_kv_len, heads, kv_heads, dim,
+                                         k_stride, _ptr(mask)))
+
+    def attention_decode_weights(self, q, k, v, o, weight, kv_len, max_kv_len, heads, kv_heads, dim, k_stride,
+                                 stream=None):
+        """mako_attention_decode_weights: attention_decode that adds each key's weight to weight [batch][kv_heads][k_stride]."""
+        _check(lib().mako_attention_decode_weights(self._h, self._stream(stream), dtype_code(q), _ptr(q), _ptr(k), _ptr(v),
+                                                   _ptr(o), _ptr(weight), kv_len.numel(), _ptr(kv_len), max_kv_len,
+                                                   heads, kv_heads, dim, k_stride))
+
+    def cache_evict(self, k, v, weight, kv_len, max_kv_len, kv_heads, dim, k_stride, sinks, recent, budget, k_out,
+                    v_out, weight_out, out_stride, kept, new_len, stream=None):
+        """mako_cache_evict: the kept rows of each sequence into k_out, v_out, weight_out (the inputs: in place)."""
+        _check(lib().mako_cache_evict(self._h, self._stream(stream), dtype_code(k), _ptr(k), _ptr(v), _ptr(weight),
+                                      kv_len.numel(), _ptr(kv_len), max_kv_len, kv_heads, dim, k_stride, sinks, recent,
+                                      budget, _ptr(k_out), _ptr(v_out), _ptr(weight_out), out_stride, _ptr(kept),
+                                      _ptr(new_len)))
 
     def _stream(self, stream):
         """The stream given, or the current one of this context's device."""
