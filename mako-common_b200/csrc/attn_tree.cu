@@ -1,0 +1,866 @@
+// Attention for drafted tokens over a KV cache on sm_100a tensor cores (mako_attention_tree): per (sequence, kv head) the
+// rows are (token, head of the group) pairs, up to thousands of keys long and few rows high.  No counterpart in the
+// reference.
+//
+// Bound by the one read of K and V (4 * dim bytes a key and kv head, 128 rows cost 2/3 of that time in products): the
+// tensor cores work on 128-row tiles however few rows there are, and everything else is arranged around streaming the
+// cache.
+//   - Work is cut by bytes: the tiles of all (sequence, kv head, row block) segments form one line that is divided
+//     evenly over one CTA an SM, whatever the lengths; a CTA may start and end inside a segment.  Each CTA finds its place
+//     on the device from kv_len (no host synchronisation).  A segment within one CTA is written at once, the pieces of a
+//     cut one go to scratch (at most two a CTA) and tree_combine_kernel merges them by log-sum-exp.
+//   - Warp 0 streams K and V tiles by TMA through one ring in the order of use; warp 1 issues the products; warp 2
+//     loads the rows of q, warp 3 cleans the drafted values; warps 4-11 are two softmax warpgroups, a thread a row.
+//   - Up to 128 rows: the two warpgroups take alternate key tiles of the same rows, each with its own S, maximum, sum and
+//     O, and merge at the end (a split within the CTA).  More rows (WIDE): each takes 128 rows of every tile.  256-wide
+//     heads: O alone takes half of TMEM, so one warpgroup runs with two S buffers of 64 keys.
+//   - S is overwritten by P: fp16, or for bf16 the bf16 of p and of what that left over (two products, 2^-17 off instead of
+//     2^-9; the tensor pipe has the room).  Base-2 softmax; a row's maximum moves only when passed by 8.
+//   - Keys at or past the cached length are seen by mask.  Scores that are not seen are replaced, not added to, so keys may
+//     hold anything; values of those tiles are cleaned in shared memory before the product: rows behind the draft become
+//     0, and so do single values that are not finite, which the rows that do see their token get back in the epilogue.
+//
+// Every wait is bounded (clock64); on a timeout the thread records a code in p.err, waits (bounded) for its own copies and
+// products in flight, and the CTA frees its TMEM and returns.
+#include "common.cuh"
+#include "kernels.h"
+#include "tc100.cuh"
+
+namespace mako {
+namespace {
+
+using namespace tc;
+
+constexpr long long WAIT_LIMIT = 1ll << 31;  // clock cycles (~1 s)
+// Pieces whose bad-value words are kept apart: the cleaner is at most a ring of loads (10 tiles, 5 pieces of one tile)
+// ahead of the epilogue that reads them.
+constexpr uint32_t BAD_RING = 8;
+
+template <int D, bool WIDE>
+struct TreeCfg {
+    static constexpr int STREAMS = D == 256 ? 1 : 2;
+    static constexpr int NT = 128 + 128 * STREAMS;
+    static constexpr uint32_t TK = D == 256 ? 64 : 128;         // keys a tile
+    static constexpr uint32_t ROWS = WIDE ? 256 : 128;          // rows a segment
+    static constexpr uint32_t KBOX = TK * 128, QBOX = 128 * 128;  // 64 values of TK keys, of 128 rows
+    static constexpr uint32_t SLOT = TK * D * 2;                // a K or V tile
+    static constexpr uint32_t NS = D == 64 ? 10 : 5;            // ring slots
+    static constexpr uint32_t QTILE = 128 * D * 2;
+    static constexpr uint32_t Q = 0, RING = Q + (WIDE ? 2 : 1) * QTILE, MISC = RING + NS * SLOT;
+    // barriers, the bad-value words, the merge of the two streams (narrow)
+    static constexpr uint32_t BAD = MISC + 512, XCHG = BAD + BAD_RING * 32;
+    static constexpr uint32_t TOTAL = XCHG + (STREAMS == 2 && !WIDE ? 2 * 128 * 8 : 0) + 1024;
+    static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+struct __align__(64) TreeParams {
+    CUtensorMap tk, tv;
+    const void* q;
+    const void* v;
+    void* o;
+    float* o_part;    // [2 * grid][ROWS][D]
+    float2* ml_part;  // [2 * grid][ROWS]: (max in log2 units, sum)
+    const int32_t* kv_len;
+    const int32_t* n_new;
+    const uint32_t* mask;
+    int* err;
+    uint64_t k_hstride;  // values a kv head of the cache
+    uint32_t batch, n_tok, heads, kv_heads, group, max_len, o_type, grid, min_units;
+    float scale_log2;
+};
+
+__device__ __forceinline__ uint32_t seq_cached(const TreeParams& p, uint32_t b)
+{
+    const int32_t l = __ldg(p.kv_len + b);
+    return l > 0 ? min(uint32_t(l), p.max_len) : 0u;
+}
+__device__ __forceinline__ uint32_t seq_drafted(const TreeParams& p, uint32_t b)
+{
+    if (!p.n_new)
+        return p.n_tok;
+    const int32_t n = __ldg(p.n_new + b);
+    return n > 0 ? min(uint32_t(n), p.n_tok) : 0u;
+}
+
+// The line of key tiles: sequence b holds kv_heads * rb segments (row blocks fastest) of `tiles` tiles each.
+struct SeqUnits {
+    uint32_t cached, drafted, tiles, rb;
+    __device__ uint32_t units(const TreeParams& p) const { return tiles * rb * p.kv_heads; }
+};
+template <uint32_t TK, uint32_t ROWS>
+__device__ __forceinline__ SeqUnits seq_units(const TreeParams& p, uint32_t b)
+{
+    SeqUnits s;
+    s.cached = seq_cached(p, b);
+    s.drafted = seq_drafted(p, b);
+    s.tiles = (s.cached + s.drafted + TK - 1) / TK;
+    s.rb = (p.group * s.drafted + ROWS - 1) / ROWS;
+    return s;
+}
+// Units before sequence b (b == batch: all of them).  Warp-collective.
+template <uint32_t TK, uint32_t ROWS>
+__device__ __forceinline__ uint64_t units_before(const TreeParams& p, uint32_t b)
+{
+    uint64_t sum = 0;
+    for (uint32_t i = threadIdx.x & 31; i < b; i += 32)
+        sum += seq_units<TK, ROWS>(p, i).units(p);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+__device__ __forceinline__ uint64_t units_per_cta(const TreeParams& p, uint64_t total)
+{
+    const uint64_t per = (total + p.grid - 1) / p.grid;
+    return per > p.min_units ? per : p.min_units;
+}
+
+// One CTA's walk over its part of the line, segment piece by segment piece; every role walks alike.
+struct Walk {
+    uint32_t b;      // sequence
+    uint32_t rem;    // units of it before this place
+    uint32_t left;   // units this CTA has left
+    bool first;      // the piece starts at the CTA's first unit
+};
+struct Piece {
+    uint32_t b, kvh, rblk, t0, nb, tiles, cached, drafted, slot;
+    bool whole;
+};
+template <uint32_t TK, uint32_t ROWS>
+__device__ __forceinline__ bool next_piece(const TreeParams& p, Walk& w, Piece& x)
+{
+    while (w.left && w.b < p.batch) {
+        const SeqUnits s = seq_units<TK, ROWS>(p, w.b);
+        if (w.rem >= s.units(p)) {
+            ++w.b;
+            w.rem = 0;
+            continue;
+        }
+        const uint32_t seg = w.rem / s.tiles;
+        x.b = w.b;
+        x.kvh = seg / s.rb;
+        x.rblk = seg % s.rb;
+        x.t0 = w.rem % s.tiles;
+        x.nb = min(s.tiles - x.t0, w.left);
+        x.tiles = s.tiles;
+        x.cached = s.cached;
+        x.drafted = s.drafted;
+        x.whole = x.nb == s.tiles;
+        x.slot = 2 * blockIdx.x + (w.first ? 0 : 1);
+        w.rem += x.nb;
+        w.left -= x.nb;
+        w.first = false;
+        return true;
+    }
+    return false;
+}
+
+// Ring positions, from the piece's first, of its tile t's K and V: K0 V0 K1 V1 ... when every tile serves both
+// streams (WIDE); K0 K1 V0 K2 V1 K3 ... when tiles alternate between S buffers.
+template <bool WIDE>
+__device__ __forceinline__ uint32_t k_at(uint32_t t)
+{
+    return WIDE ? 2 * t : t < 2 ? t : 2 * t - 1;
+}
+template <bool WIDE>
+__device__ __forceinline__ uint32_t v_at(uint32_t t, uint32_t nb)
+{
+    return WIDE ? 2 * t + 1 : nb == 1 ? 1 : 2 + t + min(t, nb - 2);
+}
+
+// 32 visibility bits of drafted keys first .. first + 31 (first may be negative: cached keys, seen by all) for token
+// tok of sequence b with `drafted` tokens.
+__device__ __forceinline__ uint32_t mask_word(const TreeParams& p, uint32_t b, uint32_t tok, uint32_t w)
+{
+    if (!p.mask)
+        return tok >= 32 * w + 31 ? 0xFFFFFFFFu : tok < 32 * w ? 0u : (2u << (tok - 32 * w)) - 1u;
+    const uint32_t nw = (p.n_tok + 31) / 32;
+    return w < nw ? __ldg(p.mask + (uint64_t(b) * p.n_tok + tok) * nw + w) : 0u;
+}
+__device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, uint32_t b, uint32_t tok, uint32_t drafted, int first)
+{
+    if (first <= -32)
+        return 0xFFFFFFFFu;
+    if (first >= int(drafted))
+        return 0u;
+    const uint32_t ahead = drafted - uint32_t(max(first, 0));  // drafted keys from max(first, 0) on
+    uint32_t x;
+    if (first < 0) {
+        x = mask_word(p, b, tok, 0);
+        if (ahead < 32)
+            x &= (1u << ahead) - 1u;
+        return x << -first | ((1u << -first) - 1u);
+    }
+    const uint32_t w = uint32_t(first) / 32, sh = uint32_t(first) % 32;
+    x = __funnelshift_r(mask_word(p, b, tok, w), sh ? mask_word(p, b, tok, w + 1) : 0u, sh);
+    return ahead < 32 ? x & ((1u << ahead) - 1u) : x;
+}
+__device__ __forceinline__ bool token_sees(const TreeParams& p, uint32_t b, uint32_t tok, uint32_t j)
+{
+    return mask_word(p, b, tok, j / 32) >> (j % 32) & 1u;
+}
+
+// The bits of the pair's 16-bit values that are not finite.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite(uint32_t u)
+{
+    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+    uint32_t m = (u & e) == e ? 0xFFFFu : 0u;
+    if ((u >> 16 & e) == e)
+        m |= 0xFFFF0000u;
+    return m;
+}
+
+template <int D, bool BF, bool WIDE>
+__global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(const __grid_constant__ TreeParams p)
+{
+    using C = TreeCfg<D, WIDE>;
+    constexpr uint32_t TK = C::TK, ROWS = C::ROWS, NS = C::NS, SC = TK;  // SC: TMEM columns of an S buffer
+    constexpr uint32_t COLO = 256;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw);
+    const uint32_t sQ = base + C::Q, sR = base + C::RING, sB = base + C::MISC;
+    auto full = [&](uint32_t s) { return sB + 8 * s; };
+    auto empty = [&](uint32_t s) { return sB + 80 + 8 * s; };
+    auto v_raw = [&](uint32_t s) { return sB + 160 + 8 * s; };  // a V tile that the cleaner still has to pass on
+    auto s_full = [&](uint32_t x) { return sB + 240 + 8 * x; };
+    auto p_full = [&](uint32_t x) { return sB + 256 + 8 * x; };
+    auto pv_done = [&](uint32_t x) { return sB + 272 + 8 * x; };
+    const uint32_t q_full = sB + 288, q_empty = sB + 296, mma_done = sB + 304;
+    volatile uint32_t* const plan = reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 320);  // b, rem, left, tmem
+    volatile uint32_t* const dead = plan + 4;  // a softmax warp gave up
+    uint32_t* const bad = reinterpret_cast<uint32_t*>(smem + C::BAD);
+    float2* const xchg = reinterpret_cast<float2*>(smem + C::XCHG);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the combine may be scheduled now
+    if (threadIdx.x == 32) {
+        for (uint32_t s = 0; s < NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+            mbar_init(v_raw(s), 1);
+        }
+        for (uint32_t x = 0; x < 2; ++x) {
+            mbar_init(s_full(x), 1);
+            mbar_init(p_full(x), 128);
+            mbar_init(pv_done(x), 1);
+        }
+        mbar_init(q_full, 32);
+        mbar_init(q_empty, 1);
+        mbar_init(mma_done, 1);
+        *dead = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) {
+        tmem_alloc(base + C::MISC + 332, 512);
+        tmem_relinquish();
+    }
+    if (warp == 0) {
+        // this CTA's part of the line: [u0, u1), then the sequence u0 lies in
+        const uint64_t total = units_before<TK, ROWS>(p, p.batch), per = units_per_cta(p, total);
+        const uint64_t u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
+        uint64_t at = 0;
+        uint32_t b = 0, rem = 0;
+        for (uint32_t i0 = 0; i0 < p.batch && u0 < u1; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const uint64_t n = i < p.batch ? seq_units<TK, ROWS>(p, i).units(p) : 0;
+            uint64_t incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o)
+                    incl += y;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, at + incl > u0);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                b = i0 + l;
+                rem = uint32_t(u0 - at - __shfl_sync(0xffffffffu, incl - n, l));
+                break;
+            }
+            at += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            plan[0] = b;
+            plan[1] = rem;
+            plan[2] = uint32_t(u1 - u0);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = plan[3];
+    Walk w{plan[0], plan[1], plan[2], true};
+    Piece x;
+    bool ok = true;
+    uint32_t n0 = 0;  // ring position of the piece's first tile
+
+    if (warp < 4) {
+        if constexpr (C::STREAMS == 2)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n" ::: "memory");
+        if (warp == 0 && lane == 0) {
+            // ---------------- TMA producer ----------------
+            tma_prefetch_desc(&p.tk);
+            tma_prefetch_desc(&p.tv);
+            uint32_t loads = 0;
+            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+                const int hd = int(x.b * p.kv_heads + x.kvh);
+                // loads in ring order
+                for (uint32_t i = 0; i < 2 * x.nb; ++i) {
+                    bool is_k;
+                    uint32_t t;
+                    if (WIDE) {
+                        is_k = (i & 1) == 0;
+                        t = i / 2;
+                    } else if (i < min(x.nb, 2u)) {
+                        is_k = true;
+                        t = i;
+                    } else if (x.nb == 1) {
+                        is_k = false;
+                        t = 0;
+                    } else {
+                        // V0 K2 V1 K3 ... V(nb-3) K(nb-1) V(nb-2) V(nb-1)
+                        const uint32_t j = i - 2;
+                        is_k = (j & 1) && j / 2 + 2 < x.nb;
+                        t = j < 2 * (x.nb - 2) ? j / 2 + (is_k ? 2 : 0) : j - (x.nb - 2);
+                    }
+                    const uint32_t n = n0 + i, s = n % NS;
+                    if (n >= NS && !mbar_wait(empty(s), (n / NS + 1) & 1, WAIT_LIMIT)) {
+                        ok = false;
+                        break;
+                    }
+                    // V tiles past the cached keys arrive at the cleaner, which passes them on to `full`
+                    const uint32_t bar = !is_k && (x.t0 + t + 1) * TK > x.cached ? v_raw(s) : full(s);
+                    mbar_expect_tx(bar, C::SLOT);
+                    for (uint32_t c = 0; c < D / 64; ++c)
+                        tma_load_3d(sR + s * C::SLOT + c * C::KBOX, is_k ? &p.tk : &p.tv, bar, c * 64,
+                                    int((x.t0 + t) * TK), hd);
+                    loads = n + 1;
+                }
+                n0 += 2 * x.nb;
+            }
+            if (!ok) {
+                atomicExch(p.err, 41);
+                // the copies in flight, the last NS loads at most, land before the CTA leaves
+                for (uint32_t n = loads > NS ? loads - NS : 0; n < loads; ++n)
+                    mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT);
+            }
+        } else if (warp == 1 && lane == 0) {
+            // ---------------- UMMA issuer ----------------
+            constexpr uint32_t F = BF ? 1u : 0u;
+            const uint32_t idesc_qk = idesc_f16(F, F, 0, 0, 128, TK);
+            const uint32_t idesc_pv = idesc_f16(F, F, 0, 1, 128, D);
+            auto qk = [&](uint32_t sbuf, uint32_t qt, uint32_t slot) {
+#pragma unroll
+                for (uint32_t ks = 0; ks < D / 16; ++ks)
+                    umma_ss(tmem + sbuf * SC, sdesc(sQ + qt * C::QTILE + (ks >> 2) * C::QBOX + (ks & 3) * 32, 16, 1024),
+                            sdesc(sR + slot * C::SLOT + (ks >> 2) * C::KBOX + (ks & 3) * 32, 16, 1024), idesc_qk, ks > 0);
+            };
+            auto pv = [&](uint32_t sbuf, uint32_t ot, uint32_t slot, bool acc) {
+#pragma unroll
+                for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
+#pragma unroll
+                    for (uint32_t kk = 0; kk < TK / 16; ++kk)
+                        umma_ts(tmem + COLO + ot * 128, tmem + sbuf * SC + part * (TK / 2) + kk * 8,
+                                sdesc(sR + slot * C::SLOT + kk * 2048, C::KBOX, 1024), idesc_pv, acc || part > 0 || kk > 0);
+            };
+            uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
+            auto wait_full = [&](uint32_t n) { return mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
+            auto wait_v = [&](uint32_t t) { return wait_full(n0 + v_at<WIDE>(t, x.nb)); };
+            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+                if (!(ok = mbar_wait(q_full, pieces & 1, WAIT_LIMIT)))
+                    break;
+                ++pieces;
+                if (WIDE) {
+                    if (!(ok = wait_full(n0)))
+                        break;
+                    fence_after();
+                    for (uint32_t y = 0; y < 2; ++y) {
+                        qk(y, y, n0 % NS);
+                        umma_commit(s_full(y));
+                    }
+                    umma_commit(empty(n0 % NS));
+                    if (x.nb == 1)
+                        umma_commit(q_empty);
+                    for (uint32_t t = 0; t < x.nb && ok; ++t) {
+                        const uint32_t vs = (n0 + 2 * t + 1) % NS, ks = (n0 + 2 * t + 2) % NS;
+                        ok = wait_v(t);
+                        for (uint32_t y = 0; y < 2 && ok; ++y) {
+                            if (!(ok = mbar_wait(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
+                                break;
+                            pc ^= 1u << y;
+                            fence_after();
+                            pv(y, y, vs, t > 0);
+                            if (y == 1)
+                                umma_commit(empty(vs));
+                            if (t + 1 < x.nb) {
+                                if (y == 0 && !(ok = wait_full(n0 + 2 * t + 2)))
+                                    break;
+                                qk(y, y, ks);
+                                umma_commit(s_full(y));
+                                if (y == 1) {
+                                    umma_commit(empty(ks));
+                                    if (t + 2 == x.nb)
+                                        umma_commit(q_empty);
+                                }
+                            } else {
+                                umma_commit(pv_done(y));
+                            }
+                        }
+                    }
+                } else {
+                    for (uint32_t t = 0; t < min(x.nb, 2u) && ok; ++t) {
+                        if (!(ok = wait_full(n0 + t)))
+                            break;
+                        fence_after();
+                        qk(t, 0, (n0 + t) % NS);
+                        umma_commit(s_full(t));
+                        umma_commit(empty((n0 + t) % NS));
+                        if (t + 1 == x.nb)
+                            umma_commit(q_empty);
+                    }
+                    for (uint32_t t = 0; t < x.nb && ok; ++t) {
+                        const uint32_t y = t & 1, vs = (n0 + v_at<WIDE>(t, x.nb)) % NS;
+                        if (!(ok = wait_v(t) && mbar_wait(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
+                            break;
+                        pc ^= 1u << y;
+                        fence_after();
+                        pv(y, C::STREAMS == 2 ? y : 0, vs, C::STREAMS == 2 ? t > 1 : t > 0);
+                        umma_commit(empty(vs));
+                        if (C::STREAMS == 1 || t + 2 >= x.nb)
+                            umma_commit(pv_done(C::STREAMS == 2 ? y : 0));
+                        if (t + 2 < x.nb) {
+                            const uint32_t kn = n0 + k_at<WIDE>(t + 2);
+                            if (!(ok = wait_full(kn)))
+                                break;
+                            qk(y, 0, kn % NS);
+                            umma_commit(s_full(y));
+                            umma_commit(empty(kn % NS));
+                            if (t + 3 == x.nb)
+                                umma_commit(q_empty);
+                        }
+                    }
+                }
+                n0 += 2 * x.nb;
+            }
+            if (!ok)
+                atomicExch(p.err, 42);
+            umma_commit(mma_done);  // every product issued above has finished before TMEM is freed
+            mbar_wait(mma_done, 0, WAIT_LIMIT);
+        } else if (warp == 2) {
+            // ---------------- q loader ----------------
+            // Rows past the drafted ones keep what the tile held: they only make rows of S and O that nobody reads.
+            constexpr uint32_t CH = D / 8, RPI = 32 / CH ? 32 / CH : 1;  // 16-byte chunks a row, rows a warp at once
+            uint32_t pieces = 0;
+            const uint16_t* const q = static_cast<const uint16_t*>(p.q);
+            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+                if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
+                    break;
+                const uint32_t rows = min(ROWS, p.group * x.drafted - x.rblk * ROWS), c = lane % CH;
+                uint32_t r = lane / CH, tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
+                for (; r < rows; r += RPI) {
+                    const uint64_t src =
+                        ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + g) * D + c * 8;
+                    cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128), q + src, true);
+                    for (g += RPI; g >= p.group; g -= p.group)
+                        ++tok;
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_async_smem();
+                mbar_arrive(q_full);
+                ++pieces;
+            }
+            if (!ok && lane == 0)
+                atomicExch(p.err, 43);
+        } else if (warp == 3) {
+            // ---------------- cleaner of the drafted values ----------------
+            uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
+            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+                uint32_t* const mybad = bad + pieces++ % BAD_RING * 8;
+                if (lane < 8)
+                    mybad[lane] = 0;
+                __syncwarp();
+                const uint32_t first = x.cached / TK;  // the first tile with keys past the cached ones
+                for (uint32_t t = first > x.t0 ? first - x.t0 : 0; t < x.nb; ++t) {
+                    const uint32_t j0 = (x.t0 + t) * TK, s = (n0 + v_at<WIDE>(t, x.nb)) % NS;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(v_raw(s), used >> s & 1u, WAIT_LIMIT))))
+                        break;
+                    used ^= 1u << s;
+                    const uint32_t r0 = x.cached > j0 ? x.cached - j0 : 0;
+                    const uint32_t r1 = min(TK, x.cached + x.drafted - j0);  // rows past it are no keys
+                    uint8_t* const tile = smem + C::RING + s * C::SLOT;
+                    auto chunk = [&](uint32_t i) {
+                        const uint32_t r = i / (D / 8), c = i % (D / 8);
+                        return reinterpret_cast<uint4*>(tile + (c >> 3) * C::KBOX + swz(r, c & 7, 128));
+                    };
+                    for (uint32_t i = r0 * (D / 8) + lane; i < r1 * (D / 8); i += 32) {
+                        uint4* const e = chunk(i);
+                        const uint4 u = *e;
+                        const uint4 m = make_uint4(not_finite<BF>(u.x), not_finite<BF>(u.y), not_finite<BF>(u.z),
+                                                   not_finite<BF>(u.w));
+                        if (m.x | m.y | m.z | m.w) {
+                            *e = make_uint4(u.x & ~m.x, u.y & ~m.y, u.z & ~m.z, u.w & ~m.w);
+                            const uint32_t j = j0 + i / (D / 8) - x.cached;
+                            atomicOr(&mybad[j / 32], 1u << (j % 32));
+                        }
+                    }
+                    for (uint32_t i = r1 * (D / 8) + lane; i < TK * (D / 8); i += 32)
+                        *chunk(i) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(full(s));
+                }
+                n0 += 2 * x.nb;
+            }
+            if (!ok && lane == 0)
+                atomicExch(p.err, 45);
+        }
+    } else {
+        if constexpr (C::STREAMS == 2)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n" ::: "memory");
+        // ---------------- softmax and epilogue ----------------
+        const uint32_t y = (warp - 4) >> 2, ql = (warp & 3) * 32, row = ql + lane;
+        const uint32_t tl = tmem + (ql << 16);
+        const float scale = p.scale_log2;
+        uint32_t pieces = 0, sc = 0, pvn = 0;  // sc: parity of each s_full's phases, pvn: pv_done's phases so far
+        while (ok && next_piece<TK, ROWS>(p, w, x)) {
+            const uint32_t live_rows = p.group * x.drafted;
+            const uint32_t rbase = x.rblk * ROWS + (WIDE ? y * 128 : 0), r = rbase + row;
+            const bool live = r < live_rows, warp_live = rbase + ql < live_rows;
+            const uint32_t tok = min(r, live_rows - 1) / p.group;
+            float m = -INFINITY, l = 0.0f;
+            uint32_t mine = 0;  // tiles of this stream so far
+            const uint32_t step = WIDE || C::STREAMS == 1 ? 1 : 2;
+            for (uint32_t t = WIDE || C::STREAMS == 1 ? 0 : y; t < x.nb; t += step, ++mine) {
+                const uint32_t sb = WIDE ? y : t & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(s_full(sb), sc >> sb & 1u, WAIT_LIMIT));
+                if (!ok)
+                    break;
+                sc ^= 1u << sb;
+                fence_after();
+                if (warp_live) {
+                    uint32_t s[TK / 32][32];
+                    if constexpr (TK == 128)
+                        tmem_ld128(tl + sb * SC, s);
+                    else
+                        tmem_ld64(tl + sb * SC, s);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (uint32_t c = 0; c < TK / 32; ++c)
+                        reg_fence(s[c]);
+                    const uint32_t j0 = (x.t0 + t) * TK;
+                    if (j0 + TK > x.cached) {
+#pragma unroll
+                        for (uint32_t c = 0; c < TK / 32; ++c) {
+                            const uint32_t bits = seen_bits(p, x.b, tok, x.drafted, int(j0 + c * 32) - int(x.cached));
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(bits >> e & 1u))
+                                    s[c][e] = 0xFF800000u;  // -inf
+                        }
+                    }
+                    float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (uint32_t c = 0; c < TK; c += 8)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e)
+                            mq[e] = max3f(mq[e], __uint_as_float(s[(c + 2 * e) >> 5][(c + 2 * e) & 31]),
+                                          __uint_as_float(s[(c + 2 * e + 1) >> 5][(c + 2 * e + 1) & 31]));
+                    const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * scale;
+                    float f = 1.0f;
+                    bool resc = false;
+                    if (mx > m + 8.0f) {
+                        f = m == -INFINITY ? 0.0f : ex2(m - mx);
+                        m = mx;
+                        l *= f;
+                        resc = true;
+                    }
+                    const float mneg = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t scale2 = pack2(scale, scale), mneg2 = pack2(mneg, mneg);
+                    uint64_t sum2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+                    for (uint32_t c = 0; c < TK / 32; ++c) {
+                        // 32 scores -> 16 columns of P (and of what rounding left over)
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float a, b;
+                            unpack2(ffma2(pack2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), scale2, mneg2),
+                                    a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum2[e & 1] = fadd2(sum2[e & 1], pack2(a, b));
+                            if (BF) {
+                                hi[e] = Elem<__nv_bfloat16>::pack(a, b);
+                                lo[e] = Elem<__nv_bfloat16>::pack(a - __uint_as_float(hi[e] << 16),
+                                                                  b - __uint_as_float(hi[e] & 0xFFFF0000u));
+                            } else {
+                                hi[e] = Elem<__half>::pack(a, b);
+                            }
+                        }
+                        tmem_st16(tl + sb * SC + c * 16, hi);
+                        if (BF)
+                            tmem_st16(tl + sb * SC + TK / 2 + c * 16, lo);
+                    }
+                    {
+                        float s0, s1, s2, s3;
+                        unpack2(sum2[0], s0, s1);
+                        unpack2(sum2[1], s2, s3);
+                        l += (s0 + s1) + (s2 + s3);
+                    }
+                    // Rescale O before the next product adds to it.  Two streams: the product before was committed
+                    // with this S.  One stream: wait for it here.
+                    if (__any_sync(0xffffffffu, resc && mine > 0)) {
+                        if (C::STREAMS == 1)
+                            ok = __all_sync(0xffffffffu, mbar_wait(pv_done(0), (pvn + mine - 1) & 1, WAIT_LIMIT));
+                        fence_after();
+                        const float gsc = resc ? f : 1.0f;
+#pragma unroll
+                        for (uint32_t c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(tl + COLO + (C::STREAMS == 2 ? y * 128 : 0) + c * 32, o);
+                            tmem_wait_ld();
+                            reg_fence(o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * gsc);
+                            tmem_st32(tl + COLO + (C::STREAMS == 2 ? y * 128 : 0) + c * 32, o);
+                        }
+                    }
+                    tmem_wait_st();
+                }
+                fence_before();
+                mbar_arrive(p_full(sb));
+                if (!ok)
+                    break;
+            }
+            // the stream's last product (one stream: every product commits pv_done)
+            if (ok && mine > 0) {
+                const uint32_t ph = C::STREAMS == 1 ? pvn + x.nb - 1 : pvn;
+                // one stream: the last S was committed with the product two tiles before, so two phases may be due
+                if (C::STREAMS == 1 && x.nb > 1)
+                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done(0), (ph - 1) & 1, WAIT_LIMIT));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(pv_done(C::STREAMS == 2 ? y : 0), ph & 1, WAIT_LIMIT));
+                fence_after();
+                pvn += C::STREAMS == 1 ? x.nb : 1;
+            }
+            // ---- epilogue: the rows' o, or their part of it
+            const uint32_t* const mybad = bad + pieces % BAD_RING * 8;
+            ++pieces;
+            float f0 = 1.0f, f1 = 0.0f;  // weights of the two streams' parts (narrow)
+            bool have1 = false;
+            constexpr bool MERGE = C::STREAMS == 2 && !WIDE;
+            if (MERGE) {
+                xchg[y * 128 + row] = make_float2(m, l);
+                if (!ok)
+                    *dead = 1;
+                named_bar(1, 256);
+                ok = *dead == 0;  // a warp that gave up ends the walk of all, which meet at these barriers
+                const float2 a = xchg[row], b = xchg[128 + row];
+                const float M = fmaxf(a.x, b.x);
+                f0 = a.x == -INFINITY ? 0.0f : ex2(a.x - M);
+                f1 = b.x == -INFINITY ? 0.0f : ex2(b.x - M);
+                have1 = x.nb > 1;
+                m = M;
+                l = have1 ? a.y * f0 + b.y * f1 : a.y * f0;
+            }
+            if (ok && warp_live) {
+                const float inv = x.whole ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+                const uint32_t lrow = (WIDE ? y * 128 : 0) + row;
+                void* dst = x.whole ? p.o : static_cast<void*>(p.o_part);
+                const uint64_t doff =
+                    x.whole ? ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + r % p.group) * D
+                            : (uint64_t(x.slot) * ROWS + lrow) * D;
+                if (!x.whole && live && (!MERGE || y == 0))
+                    p.ml_part[uint64_t(x.slot) * ROWS + lrow] = make_float2(m, l);
+                uint32_t any_bad = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    any_bad |= mybad[i];
+                // narrow: this warpgroup's half of the columns, of both parts
+                constexpr uint32_t NC = MERGE ? D / 64 : D / 32;
+#pragma unroll
+                for (uint32_t cc = 0; cc < NC; ++cc) {
+                    const uint32_t c = MERGE ? y * NC + cc : cc;
+                    uint32_t o[32];
+                    tmem_ld32(tl + COLO + (WIDE ? y * 128 : 0) + c * 32, o);
+                    tmem_wait_ld();
+                    reg_fence(o);
+                    if (MERGE) {
+                        uint32_t o1[32];
+                        if (have1) {
+                            tmem_ld32(tl + COLO + 128 + c * 32, o1);
+                            tmem_wait_ld();
+                            reg_fence(o1);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            float z = __uint_as_float(o[e]) * f0;
+                            if (have1)
+                                z = fmaf(__uint_as_float(o1[e]), f1, z);
+                            o[e] = __float_as_uint(z);
+                        }
+                    }
+                    if (any_bad) {
+                        for (uint32_t i = 0; i < 8; ++i)
+                            for (uint32_t bits = mybad[i]; bits; bits &= bits - 1) {
+                                const uint32_t j = i * 32 + __ffs(bits) - 1;
+                                if (!token_sees(p, x.b, tok, j))
+                                    continue;
+                                const uint16_t* v = static_cast<const uint16_t*>(p.v) +
+                                                    (uint64_t(x.b) * p.kv_heads + x.kvh) * p.k_hstride +
+                                                    uint64_t(x.cached + j) * D + c * 32;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    const float u = BF ? __uint_as_float(uint32_t(v[e]) << 16)
+                                                       : __half2float(__ushort_as_half(v[e]));
+                                    if (!isfinite(u))
+                                        o[e] = __float_as_uint(__uint_as_float(o[e]) + u);
+                                }
+                            }
+                    }
+                    if (live)
+                        out_store32(dst, doff + c * 32, o, inv, x.whole ? p.o_type : 0u);
+                }
+            }
+            fence_before();
+            if (MERGE)
+                named_bar(1, 256);  // both have read both parts: the next piece's products may overwrite them
+        }
+        if (!ok && lane == 0)
+            atomicExch(p.err, 44);
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// A warp a row: merges the pieces of a segment that several CTAs worked on.  Reads what the pieces wrote, nothing for
+// segments written whole.
+constexpr uint32_t CMB_WARPS = 8;
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p)
+{
+    using C = TreeCfg<D, WIDE>;
+    constexpr uint32_t V = D / 32;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const uint32_t lane = threadIdx.x & 31, b = blockIdx.y, per_kv = p.group * p.n_tok;
+    const uint32_t i = blockIdx.x * CMB_WARPS + (threadIdx.x >> 5);
+    if (i >= per_kv * p.kv_heads)
+        return;
+    const uint32_t kvh = i / per_kv, r = i % per_kv;
+    const SeqUnits s = seq_units<C::TK, C::ROWS>(p, b);
+    if (r >= p.group * s.drafted)
+        return;
+    const uint64_t per = units_per_cta(p, units_before<C::TK, C::ROWS>(p, p.batch));
+    const uint64_t u0 = units_before<C::TK, C::ROWS>(p, b) + uint64_t(kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
+    const uint32_t c0 = uint32_t(u0 / per), c1 = uint32_t((u1 - 1) / per);
+    if (c0 == c1)
+        return;
+    const uint32_t lrow = r % C::ROWS, slot0 = 2 * c0 + (u0 % per ? 1 : 0);
+    auto at = [&](uint32_t c) { return uint64_t(c == c0 ? slot0 : 2 * c) * C::ROWS + lrow; };
+    float M = -INFINITY;
+    for (uint32_t c = c0 + lane; c <= c1; c += 32)
+        M = fmaxf(M, p.ml_part[at(c)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float l = 0.0f, acc[V];
+#pragma unroll
+    for (uint32_t e = 0; e < V; ++e)
+        acc[e] = 0.0f;
+    for (uint32_t c = c0; c <= c1; ++c) {
+        const uint64_t a = at(c);
+        const float2 ml = p.ml_part[a];
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        l += ml.y * f;
+        const float* src = p.o_part + a * D + lane * V;
+#pragma unroll
+        for (uint32_t e = 0; e < V; e += 2) {
+            const float2 z = *reinterpret_cast<const float2*>(src + e);
+            acc[e] = fmaf(z.x, f, acc[e]);
+            acc[e + 1] = fmaf(z.y, f, acc[e + 1]);
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t o = ((uint64_t(b) * p.n_tok + r / p.group) * p.heads + kvh * p.group + r % p.group) * D + lane * V;
+#pragma unroll
+    for (uint32_t e = 0; e < V; e += 2)
+        out_store2(p.o, o + e, acc[e] * inv, acc[e + 1] * inv, p.o_type);
+}
+
+template <int D, bool WIDE>
+cudaError_t launch_tree_t(const TreeArgs& a, bool bf, int* err, cudaStream_t st)
+{
+    using C = TreeCfg<D, WIDE>;
+    TreeParams p;
+    if (!tile_map(&p.tk, a.k, bf, D, a.k_stride, a.batch * a.kv_heads, C::TK) ||
+        !tile_map(&p.tv, a.v, bf, D, a.k_stride, a.batch * a.kv_heads, C::TK))
+        return cudaErrorInvalidValue;
+    p.q = a.q;
+    p.v = a.v;
+    p.o = a.o;
+    p.o_part = a.o_part;
+    p.ml_part = a.ml_part;
+    p.kv_len = a.kv_len;
+    p.n_new = a.n_new;
+    p.mask = a.mask;
+    p.err = err;
+    p.k_hstride = uint64_t(a.k_stride) * D;
+    p.batch = a.batch;
+    p.n_tok = a.n_tok;
+    p.heads = a.heads;
+    p.kv_heads = a.kv_heads;
+    p.group = a.heads / a.kv_heads;
+    p.max_len = a.max_len;
+    p.o_type = a.o_type;
+    p.grid = a.ctas;
+    p.min_units = 2;
+    p.scale_log2 = a.scale * kLog2e;
+    auto kern = bf ? tree_tc_kernel<D, true, WIDE> : tree_tc_kernel<D, false, WIDE>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
+    if (e != cudaSuccess)
+        return e;
+    kern<<<a.ctas, C::NT, C::TOTAL, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess)
+        return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((p.group * p.n_tok * p.kv_heads + CMB_WARPS - 1) / CMB_WARPS, p.batch);
+    cfg.blockDim = dim3(CMB_WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_combine_kernel<D, WIDE>, p);
+}
+
+} // namespace
+
+// Rows a segment: 128, or 256 where the heads are narrow enough for two 128-row O tiles in TMEM and there are more rows.
+uint32_t tree_rows(uint32_t n_tok, uint32_t group, uint32_t dim) { return dim < 256 && n_tok * group > 128 ? 256 : 128; }
+
+cudaError_t launch_tree(const TreeArgs& a, int dtype, int dim, int* err, cudaStream_t st)
+{
+    const bool bf = dtype == kBF16, wide = tree_rows(a.n_tok, a.heads / a.kv_heads, dim) == 256;
+    switch (dim) {
+    case 64:
+        return wide ? launch_tree_t<64, true>(a, bf, err, st) : launch_tree_t<64, false>(a, bf, err, st);
+    case 128:
+        return wide ? launch_tree_t<128, true>(a, bf, err, st) : launch_tree_t<128, false>(a, bf, err, st);
+    case 256:
+        return launch_tree_t<256, false>(a, bf, err, st);
+    default:
+        return cudaErrorInvalidValue;
+    }
+}
+
+} // namespace mako

@@ -9,10 +9,8 @@
 // mma.sync (the group's q rows padded to 16), keeps its own running softmax and accumulator, and the warps merge at
 // the end into one partial (o unnormalised, max, sum) per (sequence, head, split); a sequence with one split writes
 // o directly.
-// The same kernel serves two more calls: with SCORES it also stores every scaled score, from which
-// decode_weights_kernel makes the keys' attention weights once the row's maximum and sum are known; with TREE the rows
-// of a kv head are the drafted tokens times the group's heads, and the drafted keys behind the cached ones are seen by
-// mask.
+// With SCORES the same kernel also stores every scaled score, from which decode_weights_kernel makes the keys'
+// attention weights once the row's maximum and sum are known.
 // Kernel 2 (decode_combine_kernel): the log-sum-exp merge of a row's splits into o, launched as a programmatic
 // dependent of kernel 1 so that its launch overlaps kernel 1's last wave.
 #include "common.cuh"
@@ -28,8 +26,6 @@ namespace {
 constexpr int DBN = 64, DNT = 128, DST = 3, QR = 16;
 constexpr uint64_t kMaxSplits = 1024;
 
-enum Mode { PLAIN, SCORES, TREE };
-
 // Keys of sequence b: its kv_len entry (<= 0: none) capped at max_kv_len, so that a length beyond the split plan's
 // reach is cut at max_kv_len and every kernel of a call agrees on the same split count; without kv_len, p.len.
 __device__ __forceinline__ uint32_t seq_keys(const DecodeParams& p, uint32_t b)
@@ -40,30 +36,14 @@ __device__ __forceinline__ uint32_t seq_keys(const DecodeParams& p, uint32_t b)
     return l > 0 ? min(uint32_t(l), p.len) : 0u;
 }
 
-// Drafted tokens of sequence b (TREE).
-__device__ __forceinline__ uint32_t seq_new(const DecodeParams& p, uint32_t b)
-{
-    if (!p.n_new)
-        return p.n_tok;
-    const int32_t n = p.n_new[b];
-    return n > 0 ? min(uint32_t(n), p.n_tok) : 0u;
-}
-// Whether token tok of sequence b sees drafted token j (TREE).
-__device__ __forceinline__ bool tree_sees(const DecodeParams& p, uint32_t b, uint32_t tok, uint32_t j)
-{
-    if (!p.mask)
-        return j <= tok;
-    return __ldg(p.mask + (uint64_t(b) * p.n_tok + tok) * ((p.n_tok + 31) / 32) + j / 32) >> (j % 32) & 1u;
-}
-
-// A row's value: 0 for a row that sees no key; a NaN sum stays NaN (MODE != PLAIN).
-template <int MODE>
+// A row's value: 0 for a row that sees no key; with SCORES a NaN sum stays NaN.
+template <bool SCORES>
 __device__ __forceinline__ float row_value(float o, float l)
 {
-    return (MODE == PLAIN ? l > 0.0f : l != 0.0f) ? o / l : 0.0f;
+    return (SCORES ? l != 0.0f : l > 0.0f) ? o / l : 0.0f;
 }
 
-template <int D, typename T, int MODE>
+template <int D, typename T, bool SCORES>
 __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams p)
 {
     constexpr int ROWB = D * 2, CH = D / 8, KS = D / 16, TILE = DBN * ROWB;
@@ -71,29 +51,16 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t sQ = smem_u32(smem), sK = sQ + QR * ROWB, sV = sK + DST * TILE;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3, mi = lane >> 3;
-    const uint32_t group = p.heads / p.kv_heads, rows = MODE == TREE ? group * p.n_tok : group, rb = (rows + QR - 1) / QR;
+    const uint32_t group = p.heads / p.kv_heads, rb = (group + QR - 1) / QR;
     const uint32_t b = blockIdx.z, kvh = blockIdx.y / rb, rblk = blockIdx.y % rb, split = blockIdx.x;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the combine may be scheduled now
-    const uint32_t cached = seq_keys(p, b), drafted = MODE == TREE ? seq_new(p, b) : 0u, L = cached + drafted;
+    const uint32_t L = seq_keys(p, b);
     const uint32_t start = split * p.chunk;
-    const uint32_t live = MODE == TREE ? group * drafted : group;
-    if (MODE == TREE && rblk * QR >= live)
-        return;
-    const uint32_t h0 = kvh * group + rblk * QR, nrows = min(uint32_t(QR), live - rblk * QR);
-    // the (token, head) of row r as an index into q's and o's rows
-    auto row_head = [&](uint32_t r) {
-        if (MODE != TREE)
-            return h0 + r;
-        const uint32_t t = rblk * QR + r;
-        return t / group * p.heads + kvh * group + t % group;
-    };
-    __shared__ uint32_t bad[8];  // TREE: drafted tokens of this split whose values are not all finite
-    if (MODE == TREE && tid < 8)
-        bad[tid] = 0;
+    const uint32_t h0 = kvh * group + rblk * QR, nrows = min(uint32_t(QR), group - rblk * QR);
     if (start >= L) {
         if (L == 0 && split == 0 && !p.keep_partials)  // no key: the rows are 0
             for (uint32_t i = tid; i < nrows * D; i += DNT)
-                out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(row_head(i / D)) * D + i % D, 0.0f, p.o_type);
+                out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + i / D) * D + i % D, 0.0f, p.o_type);
         return;
     }
     const uint32_t end = min(L, start + p.chunk);
@@ -104,7 +71,7 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
     for (int i = tid; i < QR * CH; i += DNT) {
         const uint32_t r = i / CH, c = i % CH;
         const bool ok = r < nrows;
-        cp_async16(sQ + swz(r, c, ROWB), qg + (ok ? uint64_t(row_head(r)) * p.q_hstride + c * 8 : 0), ok);
+        cp_async16(sQ + swz(r, c, ROWB), qg + (ok ? uint64_t(h0 + r) * p.q_hstride + c * 8 : 0), ok);
     }
     cp_async_commit();
     const uint32_t nt = (end - start + DBN - 1) / DBN;
@@ -146,21 +113,6 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
         cp_async_commit();
         const uint32_t kst = sK + (t % DST) * TILE, vst = sV + (t % DST) * TILE;
         const uint32_t kr = warp * 16;  // this warp's 16 keys of the tile
-        if (MODE == TREE && start + t * DBN + DBN > cached) {
-            // Drafted keys: a value that is not finite becomes 0 here, so that P = 0 drops it from the rows that do not
-            // see its token; the rows that do add it back at the end.
-            for (int i = tid; i < DBN * D; i += DNT) {
-                const uint32_t r = i / D, d = i % D, j = start + t * DBN + r;
-                if (j >= cached && j < end) {
-                    T* const e = reinterpret_cast<T*>(smem + QR * ROWB + DST * TILE + (t % DST) * TILE + swz(r, d / 8, ROWB)) + d % 8;
-                    if (!isfinite(Elem<T>::to_f(*e))) {
-                        *e = T(0.0f);
-                        atomicOr(&bad[(j - cached) / 32], 1u << ((j - cached) % 32));
-                    }
-                }
-            }
-            __syncthreads();
-        }
 
         float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -177,14 +129,11 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t j = jb + n * 8 + 2 * tq + (e & 1);
-                bool see = j < end;
-                if (MODE == TREE && see && j >= cached)
-                    see = tree_sees(p, b, min((rblk * QR + g + 8 * (e >> 1)) / group, p.n_tok - 1), j - cached);
-                const float x = see ? s[n][e] * scale : -INFINITY;
+                const float x = j < end ? s[n][e] * scale : -INFINITY;
                 s[n][e] = x;
                 mx[e >> 1] = fmaxf(mx[e >> 1], x);
             }
-        if (MODE == SCORES) {
+        if (SCORES) {
             // rows of s_stride (a multiple of 64) scores, so that a tile's last pair lies within its row
 #pragma unroll
             for (int r = 0; r < 2; ++r)
@@ -216,8 +165,8 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float mm = m[e >> 1];
-                // (MODE != PLAIN) a NaN score of a row with no maximum yet still makes its sum NaN
-                const float pe = mm == -INFINITY ? (MODE != PLAIN && s[n][e] != s[n][e] ? s[n][e] : 0.0f) : ex2(s[n][e] - mm);
+                // (SCORES) a NaN score of a row with no maximum yet still makes its sum NaN
+                const float pe = mm == -INFINITY ? (SCORES && s[n][e] != s[n][e] ? s[n][e] : 0.0f) : ex2(s[n][e] - mm);
                 s[n][e] = pe;
                 l[e >> 1] += pe;
             }
@@ -283,22 +232,12 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
             Ls += sm[(w * 2 + 1) * QR + r] * fw;
             O += so[(w * QR + r) * D + d] * fw;
         }
-        if (MODE == TREE) {
-#pragma unroll 1
-            for (int w = 0; w < 8; ++w)
-                for (uint32_t m = bad[w]; m; m &= m - 1) {
-                    const uint32_t j = w * 32 + __ffs(m) - 1;
-                    const float x = Elem<T>::to_f(vg[uint64_t(cached + j) * D + d]);
-                    if (!isfinite(x) && tree_sees(p, b, (rblk * QR + r) / group, j))
-                        O += x;
-                }
-        }
-        if (MODE == SCORES && d == 0 && ns == 1)
+        if (SCORES && d == 0 && ns == 1)
             p.ml_part[(uint64_t(b) * p.heads + h0 + r) * p.n_splits] = make_float2(M, Ls);
         if (ns == 1 && !p.keep_partials) {
-            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(row_head(r)) * D + d, row_value<MODE>(O, Ls), p.o_type);
+            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + r) * D + d, row_value<SCORES>(O, Ls), p.o_type);
         } else {
-            const uint64_t row = (uint64_t(b) * (MODE == TREE ? p.n_tok * p.heads : p.heads) + row_head(r)) * p.n_splits + split;
+            const uint64_t row = (uint64_t(b) * p.heads + h0 + r) * p.n_splits + split;
             p.o_part[row * D + d] = O;
             if (d == 0)
                 p.ml_part[row] = make_float2(M, Ls);
@@ -308,20 +247,18 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 
 // One CTA per (head, sequence), one thread per output value; the splits' weights 2^(m_s - M) go through shared
 // memory so each thread's loop is a stream of independent loads.
-template <int D, int MODE>
+template <int D, bool SCORES>
 __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
 {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");  // kernel 1's writes are visible from here on
     __shared__ float w[kMaxSplits];
     __shared__ float tot;
-    const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;  // TREE: h = token * heads + head
-    const uint32_t L = seq_keys(p, b) + (MODE == TREE ? seq_new(p, b) : 0u);
+    const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+    const uint32_t L = seq_keys(p, b);
     const uint32_t ns = min((L + p.chunk - 1) / p.chunk, p.n_splits);
     if (ns <= 1)  // written by kernel 1 (one split, or no key)
         return;
-    if (MODE == TREE && h / p.heads >= seq_new(p, b))
-        return;
-    const uint64_t row0 = (uint64_t(b) * gridDim.x + h) * p.n_splits;
+    const uint64_t row0 = (uint64_t(b) * p.heads + h) * p.n_splits;
     float M = -INFINITY;
     for (uint32_t s = d; s < ns; s += D)
         M = fmaxf(M, p.ml_part[row0 + s].x);
@@ -369,7 +306,7 @@ __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
     for (; s < ns; ++s)
         acc[0] += src[uint64_t(s) * D] * w[s];
     const float O = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
-    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, row_value<MODE>(O, tot), p.o_type);
+    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, row_value<SCORES>(O, tot), p.o_type);
 }
 
 // The keys' attention weights from the stored scores (SCORES): a CTA takes WKEYS keys of one kv head.  First a warp a
@@ -431,7 +368,7 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
     static_assert((4 * 2 * QR + 4 * QR * D) * 4 <= 2 * DST * DBN * D * 2, "merge buffer fits the stage ring");
-    auto kern = decode_split_kernel<D, T, PLAIN>;
+    auto kern = decode_split_kernel<D, T, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
@@ -448,18 +385,18 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, PLAIN>, p);
+    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, false>, p);
 }
 
-template <int D, typename T, int MODE>
+template <int D, typename T, bool SCORES>
 cudaError_t launch_split_only(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
-    auto kern = decode_split_kernel<D, T, MODE>;
+    auto kern = decode_split_kernel<D, T, SCORES>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
-    const uint32_t rows = p.heads / p.kv_heads * (MODE == TREE ? p.n_tok : 1u), rb = (rows + QR - 1) / QR;
+    const uint32_t group = p.heads / p.kv_heads, rb = (group + QR - 1) / QR;
     kern<<<dim3(p.n_splits, p.kv_heads * rb, p.batch), DNT, smem, st>>>(p);
     return cudaGetLastError();
 }
@@ -612,11 +549,11 @@ cudaError_t launch_decode_split(const DecodeParams& p, int dtype, int dim, cudaS
     const bool bf = dtype == kBF16;
     switch (dim) {
     case 64:
-        return bf ? launch_split_only<64, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<64, __half, PLAIN>(p, st);
+        return bf ? launch_split_only<64, __nv_bfloat16, false>(p, st) : launch_split_only<64, __half, false>(p, st);
     case 128:
-        return bf ? launch_split_only<128, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<128, __half, PLAIN>(p, st);
+        return bf ? launch_split_only<128, __nv_bfloat16, false>(p, st) : launch_split_only<128, __half, false>(p, st);
     case 256:
-        return bf ? launch_split_only<256, __nv_bfloat16, PLAIN>(p, st) : launch_split_only<256, __half, PLAIN>(p, st);
+        return bf ? launch_split_only<256, __nv_bfloat16, false>(p, st) : launch_split_only<256, __half, false>(p, st);
     default:
         return cudaErrorInvalidValue;
     }
@@ -637,11 +574,11 @@ cudaError_t launch_decode_combine(const DecodeParams& p, int dim, cudaStream_t s
     cfg.numAttrs = 1;
     switch (dim) {
     case 64:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64, PLAIN>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64, false>, p);
     case 128:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128, PLAIN>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128, false>, p);
     case 256:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256, PLAIN>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256, false>, p);
     default:
         return cudaErrorInvalidValue;
     }
@@ -664,37 +601,20 @@ cudaLaunchConfig_t dependent(dim3 grid, dim3 block, cudaStream_t st, cudaLaunchA
 }
 
 template <int D>
-cudaError_t launch_tree_d(const DecodeParams& p, bool bf, cudaStream_t st)
-{
-    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, TREE>(p, st) : launch_split_only<D, __half, TREE>(p, st);
-    if (e != cudaSuccess)
-        return e;
-    cudaLaunchAttribute attr;
-    const auto cfg = dependent(dim3(p.heads * p.n_tok, p.batch), dim3(D), st, &attr);
-    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, TREE>, p);
-}
-
-template <int D>
 cudaError_t launch_weights_d(const DecodeParams& p, bool bf, cudaStream_t st)
 {
-    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, SCORES>(p, st) : launch_split_only<D, __half, SCORES>(p, st);
+    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, true>(p, st) : launch_split_only<D, __half, true>(p, st);
     if (e != cudaSuccess)
         return e;
     cudaLaunchAttribute attr;
     auto cfg = dependent(dim3(p.heads, p.batch), dim3(D), st, &attr);
-    if ((e = cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, SCORES>, p)) != cudaSuccess || p.len == 0)
+    if ((e = cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, true>, p)) != cudaSuccess || p.len == 0)
         return e;
     cfg = dependent(dim3((p.len + WKEYS - 1) / WKEYS, p.kv_heads, p.batch), dim3(WNT), st, &attr);
     return cudaLaunchKernelEx(&cfg, decode_weights_kernel, p);
 }
 
 } // namespace
-
-cudaError_t launch_tree(const DecodeParams& p, int dtype, int dim, cudaStream_t st)
-{
-    const bool bf = dtype == kBF16;
-    return dim == 64 ? launch_tree_d<64>(p, bf, st) : dim == 128 ? launch_tree_d<128>(p, bf, st) : launch_tree_d<256>(p, bf, st);
-}
 
 cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t st)
 {

@@ -77,11 +77,6 @@ struct DecodeParams {
     float* scores;
     float* weight;
     uint64_t s_stride, w_stride;
-    // tree: rows are (token, head) pairs, q and o [batch][n_tok][heads][dim]; kv_len counts the cached keys, the
-    // drafted ones follow; o_part and ml_part have n_tok * heads rows a sequence
-    const int32_t* n_new;  // [batch] or null: n_tok
-    const uint32_t* mask;  // [batch][n_tok][(n_tok + 31) / 32] or null: a chain
-    uint32_t n_tok;
 };
 // Keys a split takes and how many splits, for the longest sequence max_len (chunk_opt: 0 automatic, else the
 // requested multiple of 64).
@@ -89,8 +84,23 @@ void decode_plan(uint32_t max_len, uint32_t batch, uint32_t kv_heads, uint32_t h
                  uint32_t* chunk, uint32_t* n_splits);
 cudaError_t launch_decode(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
 
-// Tree attention: the splits over cached and drafted keys, then the combine.
-cudaError_t launch_tree(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
+// Attention for drafted tokens over a cache: q and o [batch][n_tok][heads][dim]; kv_len counts the cached keys, the
+// drafted ones follow.
+struct TreeArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;
+    float* o_part;    // scratch [2 * ctas][tree_rows][dim]
+    float2* ml_part;  // scratch [2 * ctas][tree_rows]
+    const int32_t* kv_len;  // [batch], capped at max_len
+    const int32_t* n_new;   // [batch] or null: n_tok
+    const uint32_t* mask;   // [batch][n_tok][(n_tok + 31) / 32] or null: a chain
+    uint32_t max_len, batch, n_tok, heads, kv_heads, k_stride, o_type, ctas;
+    float scale;
+};
+uint32_t tree_rows(uint32_t n_tok, uint32_t group, uint32_t dim);
+cudaError_t launch_tree(const TreeArgs& a, int dtype, int dim, int* err, cudaStream_t s);
 // Decode that also adds every key's attention weight to p.weight: splits, combine, weights.
 cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
 

@@ -982,42 +982,40 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
         return MAKO_OK;
     if (!q || !k || !v || !o || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
         return fail(MAKO_EINVAL, "tree: null or unaligned tensor (16-byte alignment)");
+    if (ctx->cc_major != 10)
+        return fail(MAKO_ENOTSUP, "tree: the tcgen05 kernel needs sm_100 (sm_%d)", ctx->cc_major * 10);
     DeviceGuard dg(ctx->device);
     if (dg.err != cudaSuccess)
         return cuda_fail("set device", dg.err);
-    mako::DecodeParams p{};
-    p.q = q;
-    p.k = k;
-    p.v = v;
-    p.o = o;
-    p.kv_len = kv_len;
-    p.len = max_kv_len;
-    p.q_bstride = uint64_t(n_tok) * heads * dim;
-    p.q_hstride = dim;
-    p.k_hstride = uint64_t(k_stride) * dim;
-    p.k_bstride = uint64_t(kv_heads) * p.k_hstride;
-    p.o_bstride = p.q_bstride;
-    p.o_type = out_type(ctx, dtype);
-    p.batch = batch;
-    p.heads = heads;
-    p.kv_heads = kv_heads;
-    p.scale = 1.0f / sqrtf(float(dim));
-    p.n_new = n_new;
-    p.mask = mask;
-    p.n_tok = n_tok;
-    mako::decode_plan(max_kv_len + n_tok, batch, kv_heads, heads, ctx->num_sms, 0, &p.chunk, &p.n_splits);
-    const size_t rows = size_t(batch) * n_tok * heads * p.n_splits;
+    mako::TreeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.o = o;
+    a.kv_len = kv_len;
+    a.n_new = n_new;
+    a.mask = mask;
+    a.max_len = max_kv_len;
+    a.batch = batch;
+    a.n_tok = n_tok;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.k_stride = k_stride;
+    a.o_type = out_type(ctx, dtype);
+    a.ctas = ctx->persistent_ctas();
+    a.scale = 1.0f / sqrtf(float(dim));
+    const size_t rows = size_t(2) * a.ctas * mako::tree_rows(n_tok, heads / kv_heads, dim);
     void *op, *mlp;
     if (int rc = scratch_kept(ctx, "tree_o", rows * dim * 4, &op))
         return rc;
     if (int rc = scratch_kept(ctx, "tree_ml", rows * 8, &mlp))
         return rc;
-    p.o_part = static_cast<float*>(op);
-    p.ml_part = static_cast<float2*>(mlp);
+    a.o_part = static_cast<float*>(op);
+    a.ml_part = static_cast<float2*>(mlp);
     ctx->launches += 2;
     auto st = static_cast<cudaStream_t>(stream);
     KernelTimer t(ctx, st);
-    cudaError_t e = mako::launch_tree(p, dtype, int(dim), st);
+    cudaError_t e = mako::launch_tree(a, dtype, int(dim), ctx->err, st);
     t.stop();
     return launched("tree", e);
 }

@@ -24,7 +24,7 @@ def want_rows(q, k, v, cached, new, see, dtype):
 
 
 def run(ctx, dtype, n_tok, heads, kv_heads, dim, lens, new=None, chain=False, out16=False, seed=0, k_stride=None,
-        max_len=None, see=None):
+        max_len=None, see=None, ctas=0):
     import cache_cases as C
     import mako_attn
     import torch
@@ -41,11 +41,13 @@ def run(ctx, dtype, n_tok, heads, kv_heads, dim, lens, new=None, chain=False, ou
         see, mask = np.tril(np.ones((B, n_tok, n_tok), bool)), None
     o = torch.full((B, n_tok, heads * dim), 77.0, dtype=C.DT[dtype] if out16 else torch.float32, device="cuda")
     ctx.set_option(mako_attn.OPT_OUTPUT_16BIT, int(out16))
+    ctx.set_option(mako_attn.OPT_GRID_CTAS, ctas)
     try:
         ctx.attention_tree(q, k, v, o, B, n_tok, None if new is None else C.i32(new), C.i32(lens), top, heads, kv_heads,
                            dim, S, mask)
     finally:
         ctx.set_option(mako_attn.OPT_OUTPUT_16BIT, 0)
+        ctx.set_option(mako_attn.OPT_GRID_CTAS, 0)
     torch.cuda.synchronize()
     assert ctx.device_error() == 0
     for b in range(B):
@@ -96,6 +98,14 @@ def test_long_and_16bit(ctx, dtype):
     run(ctx, dtype, 16, 8, 2, 128, [20000, 3, 9000], out16=True)
     run(ctx, dtype, 64, 8, 2, 128, [20001, 11], out16=True)
     run(ctx, dtype, 37, 16, 2, 256, [5001, 11], out16=True)
+
+
+@pytest.mark.parametrize("ctas", [1, 2, 3, 7, 31])
+@pytest.mark.parametrize("dtype,dim,n_tok,heads", [(0, 64, 9, 4), (1, 128, 9, 8), (1, 128, 70, 8), (0, 64, 70, 4), (1, 256, 21, 8)])
+def test_few_ctas(ctx, ctas, dtype, dim, n_tok, heads):
+    """Many pieces a CTA, whole and cut at either end, of one tile and of many."""
+    run(ctx, dtype, n_tok, heads, 2, dim, [0, 1500, 3, 200, 0, 64, 127, 128, 700], new=[n_tok, 5, 1, 0, n_tok, 2, n_tok, 3, 1],
+        k_stride=1600, ctas=ctas, seed=ctas)
 
 
 def test_many_sequences(ctx):
