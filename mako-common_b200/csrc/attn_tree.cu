@@ -9,8 +9,8 @@
 //     evenly over one CTA an SM, whatever the lengths; a CTA may start and end inside a segment.  Each CTA finds its place
 //     on the device from kv_len (no host synchronisation).  A segment within one CTA is written at once, the pieces of a
 //     cut one go to scratch (at most two a CTA) and tree_combine_kernel merges them by log-sum-exp.
-//   - Warp 0 streams K and V tiles by TMA through one ring in the order of use; warp 1 issues the products; warp 2
-//     loads the rows of q, warp 3 cleans the drafted values; warps 4-11 are two softmax warpgroups, a thread a row.
+//   - Warp 0 streams K and V tiles by TMA through one ring in the order of use; warp 1 issues the products; warps 2 and
+//     3 load the rows of q, the latter cleans the drafted values; warps 4-11 are two softmax warpgroups, a thread a row.
 //   - Up to 128 rows: the two warpgroups take alternate key tiles of the same rows, each with its own S, maximum, sum and
 //     O, and merge at the end (a split within the CTA).  More rows (WIDE): each takes 128 rows of every tile.  256-wide
 //     heads: O alone takes half of TMEM, so one warpgroup runs with two S buffers of 64 keys.
@@ -96,18 +96,6 @@ __device__ __forceinline__ SeqUnits seq_units(const TreeParams& p, uint32_t b)
     s.tiles = (s.cached + s.drafted + TK - 1) / TK;
     s.rb = (p.group * s.drafted + ROWS - 1) / ROWS;
     return s;
-}
-// Units before sequence b (b == batch: all of them).  Warp-collective.
-template <uint32_t TK, uint32_t ROWS>
-__device__ __forceinline__ uint64_t units_before(const TreeParams& p, uint32_t b)
-{
-    uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x & 31; i < b; i += 32)
-        sum += seq_units<TK, ROWS>(p, i).units(p);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
 }
 __device__ __forceinline__ uint64_t units_per_cta(const TreeParams& p, uint64_t total)
 {
@@ -246,7 +234,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
             mbar_init(p_full(x), 128);
             mbar_init(pv_done(x), 1);
         }
-        mbar_init(q_full, 32);
+        mbar_init(q_full, 64);
         mbar_init(q_empty, 1);
         mbar_init(mma_done, 1);
         *dead = 0;
@@ -258,14 +246,17 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
     }
     if (warp == 0) {
         // this CTA's part of the line: [u0, u1), then the sequence u0 lies in
-        const uint64_t total = units_before<TK, ROWS>(p, p.batch), per = units_per_cta(p, total);
-        const uint64_t u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
+        uint64_t units = lane < p.batch ? seq_units<TK, ROWS>(p, lane).units(p) : 0, total = units;
+        for (uint32_t i = lane + 32; i < p.batch; i += 32)
+            total += seq_units<TK, ROWS>(p, i).units(p);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+        const uint64_t per = units_per_cta(p, total), u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
         uint64_t at = 0;
         uint32_t b = 0, rem = 0;
-        for (uint32_t i0 = 0; i0 < p.batch && u0 < u1; i0 += 32) {
-            const uint32_t i = i0 + lane;
-            const uint64_t n = i < p.batch ? seq_units<TK, ROWS>(p, i).units(p) : 0;
-            uint64_t incl = n;
+        for (uint32_t i0 = 0; u0 < u1; i0 += 32) {
+            uint64_t incl = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -276,10 +267,11 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
             if (hit) {
                 const int l = __ffs(hit) - 1;
                 b = i0 + l;
-                rem = uint32_t(u0 - at - __shfl_sync(0xffffffffu, incl - n, l));
+                rem = uint32_t(u0 - at - __shfl_sync(0xffffffffu, incl - units, l));
                 break;
             }
             at += __shfl_sync(0xffffffffu, incl, 31);
+            units = i0 + 32 + lane < p.batch ? seq_units<TK, ROWS>(p, i0 + 32 + lane).units(p) : 0;
         }
         if (lane == 0) {
             plan[0] = b;
@@ -357,12 +349,15 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                     umma_ss(tmem + sbuf * SC, sdesc(sQ + qt * C::QTILE + (ks >> 2) * C::QBOX + (ks & 3) * 32, 16, 1024),
                             sdesc(sR + slot * C::SLOT + (ks >> 2) * C::KBOX + (ks & 3) * 32, 16, 1024), idesc_qk, ks > 0);
             };
-            auto pv = [&](uint32_t sbuf, uint32_t ot, uint32_t slot, bool acc) {
+            // P.V over the tile's 16-key groups that hold keys (the cleaner has made the last group's other rows 0)
+            auto pv = [&](uint32_t sbuf, uint32_t ot, uint32_t slot, uint32_t t, bool acc) {
+                const uint32_t groups = min(TK, x.cached + x.drafted - (x.t0 + t) * TK) + 15;
 #pragma unroll
                 for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
 #pragma unroll
                     for (uint32_t kk = 0; kk < TK / 16; ++kk)
-                        umma_ts(tmem + COLO + ot * 128, tmem + sbuf * SC + part * (TK / 2) + kk * 8,
+                        if (kk < groups / 16)
+                            umma_ts(tmem + COLO + ot * 128, tmem + sbuf * SC + part * (TK / 2) + kk * 8,
                                 sdesc(sR + slot * C::SLOT + kk * 2048, C::KBOX, 1024), idesc_pv, acc || part > 0 || kk > 0);
             };
             uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
@@ -391,7 +386,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                                 break;
                             pc ^= 1u << y;
                             fence_after();
-                            pv(y, y, vs, t > 0);
+                            pv(y, y, vs, t, t > 0);
                             if (y == 1)
                                 umma_commit(empty(vs));
                             if (t + 1 < x.nb) {
@@ -426,7 +421,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                             break;
                         pc ^= 1u << y;
                         fence_after();
-                        pv(y, C::STREAMS == 2 ? y : 0, vs, C::STREAMS == 2 ? t > 1 : t > 0);
+                        pv(y, C::STREAMS == 2 ? y : 0, vs, t, C::STREAMS == 2 ? t > 1 : t > 0);
                         umma_commit(empty(vs));
                         if (C::STREAMS == 1 || t + 2 >= x.nb)
                             umma_commit(pv_done(C::STREAMS == 2 ? y : 0));
@@ -448,36 +443,35 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                 atomicExch(p.err, 42);
             umma_commit(mma_done);  // every product issued above has finished before TMEM is freed
             mbar_wait(mma_done, 0, WAIT_LIMIT);
-        } else if (warp == 2) {
-            // ---------------- q loader ----------------
+        } else if (warp >= 2) {
+            // ---------------- q loaders, the second also cleans the drafted values ----------------
             // Rows past the drafted ones keep what the tile held: they only make rows of S and O that nobody reads.
-            constexpr uint32_t CH = D / 8, RPI = 32 / CH ? 32 / CH : 1;  // 16-byte chunks a row, rows a warp at once
-            uint32_t pieces = 0;
-            const uint16_t* const q = static_cast<const uint16_t*>(p.q);
+            constexpr uint32_t CH = D / 8, RPI = 2 * (32 / CH);  // 16-byte chunks a row, rows the warps load at once
+            uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
             while (ok && next_piece<TK, ROWS>(p, w, x)) {
                 if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
                     break;
-                const uint32_t rows = min(ROWS, p.group * x.drafted - x.rblk * ROWS), c = lane % CH;
-                uint32_t r = lane / CH, tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
-                for (; r < rows; r += RPI) {
-                    const uint64_t src =
-                        ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + g) * D + c * 8;
-                    cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128), q + src, true);
-                    for (g += RPI; g >= p.group; g -= p.group)
-                        ++tok;
+                {
+                    const uint32_t rows = min(ROWS, p.group * x.drafted - x.rblk * ROWS), c = lane % CH;
+                    uint32_t r = (warp - 2) * (RPI / 2) + lane / CH;
+                    uint32_t tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
+                    const uint16_t* src = static_cast<const uint16_t*>(p.q) +
+                                          ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + g) * D + c * 8;
+                    for (; r < rows; r += RPI) {
+                        cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128), src, true);
+                        src += RPI * D;
+                        for (g += RPI; g >= p.group; g -= p.group)
+                            src += (p.heads - p.group) * D;  // the group's heads of the next token
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    fence_proxy_async_smem();
+                    mbar_arrive(q_full);
                 }
-                cp_async_commit();
-                cp_async_wait<0>();
-                fence_proxy_async_smem();
-                mbar_arrive(q_full);
-                ++pieces;
-            }
-            if (!ok && lane == 0)
-                atomicExch(p.err, 43);
-        } else if (warp == 3) {
-            // ---------------- cleaner of the drafted values ----------------
-            uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
-            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+                if (warp == 2) {
+                    ++pieces;
+                    continue;
+                }
                 uint32_t* const mybad = bad + pieces++ % BAD_RING * 8;
                 if (lane < 8)
                     mybad[lane] = 0;
@@ -506,7 +500,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                             atomicOr(&mybad[j / 32], 1u << (j % 32));
                         }
                     }
-                    for (uint32_t i = r1 * (D / 8) + lane; i < TK * (D / 8); i += 32)
+                    for (uint32_t i = r1 * (D / 8) + lane; i < (r1 + 15) / 16 * 16 * (D / 8); i += 32)
                         *chunk(i) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -516,7 +510,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                 n0 += 2 * x.nb;
             }
             if (!ok && lane == 0)
-                atomicExch(p.err, 45);
+                atomicExch(p.err, 43);
         }
     } else {
         if constexpr (C::STREAMS == 2)
@@ -742,51 +736,72 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
     }
 }
 
-// A warp a row: merges the pieces of a segment that several CTAs worked on.  Reads what the pieces wrote, nothing for
-// segments written whole.
+// A warp a row: merges the pieces of a segment that several CTAs worked on; rows of segments written whole have
+// nothing to do.  Which pieces there are follows from the lengths alone and is worked out before the wait for the main
+// kernel; the weights of 32 pieces are made at once, a lane a piece, and their rows' loads do not depend on one another.
 constexpr uint32_t CMB_WARPS = 8;
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p)
 {
     using C = TreeCfg<D, WIDE>;
     constexpr uint32_t V = D / 32;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const uint32_t lane = threadIdx.x & 31, b = blockIdx.y, per_kv = p.group * p.n_tok;
     const uint32_t i = blockIdx.x * CMB_WARPS + (threadIdx.x >> 5);
-    if (i >= per_kv * p.kv_heads)
-        return;
-    const uint32_t kvh = i / per_kv, r = i % per_kv;
+    uint64_t before = 0, total = 0;
+    for (uint32_t k = lane; k < p.batch; k += 32) {
+        const uint64_t n = seq_units<C::TK, C::ROWS>(p, k).units(p);
+        total += n;
+        before += k < b ? n : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
     const SeqUnits s = seq_units<C::TK, C::ROWS>(p, b);
-    if (r >= p.group * s.drafted)
+    const uint32_t kvh = i / per_kv, r = i % per_kv;
+    if (kvh >= p.kv_heads || r >= p.group * s.drafted)
         return;
-    const uint64_t per = units_per_cta(p, units_before<C::TK, C::ROWS>(p, p.batch));
-    const uint64_t u0 = units_before<C::TK, C::ROWS>(p, b) + uint64_t(kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
+    const uint64_t per = units_per_cta(p, total);
+    const uint64_t u0 = before + uint64_t(kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
     const uint32_t c0 = uint32_t(u0 / per), c1 = uint32_t((u1 - 1) / per);
     if (c0 == c1)
         return;
     const uint32_t lrow = r % C::ROWS, slot0 = 2 * c0 + (u0 % per ? 1 : 0);
     auto at = [&](uint32_t c) { return uint64_t(c == c0 ? slot0 : 2 * c) * C::ROWS + lrow; };
-    float M = -INFINITY;
-    for (uint32_t c = c0 + lane; c <= c1; c += 32)
-        M = fmaxf(M, p.ml_part[at(c)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float l = 0.0f, acc[V];
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    float M = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (uint32_t e = 0; e < V; ++e)
         acc[e] = 0.0f;
-    for (uint32_t c = c0; c <= c1; ++c) {
-        const uint64_t a = at(c);
-        const float2 ml = p.ml_part[a];
-        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        l += ml.y * f;
-        const float* src = p.o_part + a * D + lane * V;
+    for (uint32_t cb = c0; cb <= c1; cb += 32) {
+        const uint32_t n = min(32u, c1 - cb + 1);
+        const float2 ml = lane < n ? p.ml_part[at(cb + lane)] : make_float2(-INFINITY, 0.0f);
+        float m1 = ml.x;
 #pragma unroll
-        for (uint32_t e = 0; e < V; e += 2) {
-            const float2 z = *reinterpret_cast<const float2*>(src + e);
-            acc[e] = fmaf(z.x, f, acc[e]);
-            acc[e + 1] = fmaf(z.y, f, acc[e + 1]);
+        for (int o = 16; o > 0; o >>= 1)
+            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        const float Mn = fmaxf(M, m1), f0 = M == -INFINITY ? 0.0f : ex2(M - Mn);
+        M = Mn;
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        float ls = ml.y * f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            ls += __shfl_xor_sync(0xffffffffu, ls, o);
+        l = l * f0 + ls;
+#pragma unroll
+        for (uint32_t e = 0; e < V; ++e)
+            acc[e] *= f0;
+#pragma unroll 4
+        for (uint32_t k = 0; k < n; ++k) {
+            const float w = __shfl_sync(0xffffffffu, f, k);
+            const float* src = p.o_part + at(cb + k) * D + lane * V;
+#pragma unroll
+            for (uint32_t e = 0; e < V; e += 2) {
+                const float2 z = __ldcs(reinterpret_cast<const float2*>(src + e));
+                acc[e] = fmaf(z.x, w, acc[e]);
+                acc[e + 1] = fmaf(z.y, w, acc[e + 1]);
+            }
         }
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;

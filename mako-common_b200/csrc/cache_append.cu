@@ -132,7 +132,41 @@ __global__ void cache_append_kernel(const AppendParams p)
                         }
                     }
                 }
-            } else {  // halves: through the warp's copy of the head
+            } else if (half % VB == 0) {
+                // halves a whole number of chunks (VB values) apart: the partner of this lane's chunk is a chunk of
+                // another lane, or of the other block
+                const uint32_t hc = half / VB;
+                uint32_t from[NB];
+                float cc[VPL], sn[VPL];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const uint32_t c = n * 32 + lane;
+                    const bool first = c < hc;
+                    from[n] = first ? c + hc : c < 2 * hc ? c - hc : c;
+#pragma unroll
+                    for (int e = 0; e < VB; ++e) {
+                        const float2 a = c < 2 * hc ? cs[(first ? c : c - hc) * VB + e] : make_float2(1.0f, 0.0f);
+                        cc[n * VB + e] = a.x;
+                        sn[n * VB + e] = first ? -a.y : a.y;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < HPW; ++j) {
+                    float u[VPL];
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int e = 0; e < VB; ++e) {
+                            const float u0 = __shfl_sync(0xffffffffu, v[j][e], from[n] % 32);
+                            const float u1 = NB == 2 ? __shfl_sync(0xffffffffu, v[j][VPL - VB + e], from[n] % 32) : u0;
+                            u[n * VB + e] = from[n] < 32 ? u0 : u1;
+                        }
+#pragma unroll
+                    for (int e = 0; e < VPL; ++e)
+                        if ((e / VB) * 32 + lane < 2 * hc)
+                            v[j][e] = fmaf(v[j][e], cc[e], u[e] * sn[e]);
+                }
+            } else {  // other halves: through the warp's copy of the head
 #pragma unroll
                 for (int j = 0; j < HPW; ++j) {
                     if (uint32_t(j) >= nh)

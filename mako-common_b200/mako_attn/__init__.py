@@ -115,7 +115,7 @@ def _check(rc: int):
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream(stream):
@@ -263,8 +263,7 @@ class Context:
     def _stream(self, stream):
         """The stream given, or the current one of this context's device."""
         import torch
-        s = torch.cuda.current_stream(self.device) if stream is None else stream
-        return ctypes.c_void_p(s.cuda_stream)
+        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else stream.cuda_stream
 
     # -- TransformerRuntime::cube_select (src/models/runtime.cpp:286-303); returns (sel, nsel) as int16 tensor views
     # of the context's scratch ([heads][n_cubes][min(topk, n_cubes)] and [heads][n_cubes], uint16 bit patterns),

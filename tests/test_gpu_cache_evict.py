@@ -163,6 +163,14 @@ def test_evict_weights_of_every_kind(ctx, in_place):
                     seed=i)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_long_rows(ctx, in_place):
+    """Rows of one CTA's registers and a few more, of a cluster's, and past them."""
+    for n in (32768, 32769, 70001, 262144, 262145, 400000):
+        check_evict(ctx, 0, 1, 64, [n, 31], 5, 300, 1234, n + 1, n + 1 if in_place else 1300, in_place=in_place, seed=n)
+    check_evict(ctx, 1, 1, 64, [300000], 0, 0, 290000, 300000, 300000, weight=np.float32(0.5), in_place=in_place)
+
+
 def test_evict_capped_and_aliased_lengths(ctx):
     check_evict(ctx, 0, 2, 128, [900, 400, 1200], 4, 16, 256, 1300, 256, max_len=800)
     check_evict(ctx, 0, 4, 64, [900, 100, 1200], 4, 16, 256, 1300, 1300, in_place=True, alias_len=True)
