@@ -1,12 +1,15 @@
 // Eviction from a KV cache by accumulated attention weight (mako_cache_evict).  No counterpart in the reference.
 //
-// evict_select_kernel: a cluster of 1 to 8 CTAs a (sequence, kv head), its weights held in registers as
-// order-preserving integers (SKEYS a thread; longer rows are read again by every pass).  The rows between the sinks and
-// the recent ones compete; the weight of the last that stays is found by a radix select of 11, 11 and 10 bits: a
-// histogram in shared memory, merged over the cluster.  Equal digits in a warp are added once, so that rows of equal
-// weights do not queue at one counter.  All counts are integers: the result does not depend on the order of the adds.
-// Then every warp, which owns consecutive rows, writes its kept rows' indices from the count of those before it, ties
-// taken from the lowest row on.
+// evict_select_kernel: a CTA a (sequence, kv head), for long rows a cluster of up to 8, the weights held in registers
+// as order-preserving integers (SKEYS a thread; rows past a cluster's registers are read again by every pass).  The rows
+// between the sinks and the recent ones compete; the weight of the last that stays is found by a radix select of 11, 11
+// and 10 bits: a histogram in shared memory, merged over the cluster.  A warp whose keys all share a digit adds them at
+// once, so that rows of equal weights do not queue at one counter.  All counts are integers: the result does not depend on
+// the order of the adds.  Then every warp, which owns consecutive rows, writes its kept rows' indices from the count of
+// those before it, ties taken from the lowest row on.
+// Bound by issue: about 40 instructions a key.  24576 keys a row: 26 us with two CTAs a row, per-key warp votes around the
+// histogram and a guard on every unrolled key; a cluster barrier costs about 1500 cycles, so rows that fit one CTA's
+// registers take one.
 // evict_copy_kernel and evict_in_place_kernel copy the kept rows.  In place, row i comes from row kept[i] >= i: a CTA owns a 64-byte column
 // slice of every row and walks the rows upwards in steps, reading a whole step before it writes it, so what a later step
 // reads (rows at or past its own first) has not been written yet.
@@ -20,8 +23,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t SNT = 1024, SKEYS = 32, SBINS = 2048, MNT = 256;
-constexpr uint32_t SWARPS = SNT / 32, SMAX_CLUSTER = 8;
+constexpr uint32_t SNT = 1024, SKEYS = 32, SBINS = 2048, SMAX_CLUSTER = 8, MNT = 256;
 
 // Weights as integers of the same order; NaN below all others, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w)
@@ -44,29 +46,13 @@ __device__ __forceinline__ uint32_t warp_incl_scan(uint32_t x)
     return x;
 }
 
-// Adds one to hist[bin] for every lane that counts: once for all lanes with the first one's bin, then one by one.
-__device__ __forceinline__ void count_bin(uint32_t* hist, uint32_t bin, bool counts)
-{
-    const uint32_t lane = threadIdx.x & 31, who = __ballot_sync(0xffffffffu, counts);
-    if (!who)
-        return;
-    const int first = __ffs(who) - 1;
-    const uint32_t lead = __shfl_sync(0xffffffffu, bin, first);  // by every lane, whether it counts or not
-    const bool same = counts && bin == lead;
-    const uint32_t n = __popc(__ballot_sync(0xffffffffu, same));
-    if (int(lane) == first)
-        atomicAdd(&hist[bin], n);
-    else if (counts && !same)
-        atomicAdd(&hist[bin], 1u);
-}
-
-// REG: a thread's keys fit its SKEYS registers.
+// REG: a thread's keys fit its SKEYS registers.  blockDim.x: 256 or 1024.
 template <bool REG>
 __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
 {
-    __shared__ uint32_t hist[SBINS], sum[SBINS], part[SWARPS], found[2], mine[2], ranks[2][SWARPS];
+    __shared__ uint32_t hist[SBINS], sum[SBINS], part[32], mine[2], ranks[2][32];
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank(), nt = blockDim.x, warps = nt / 32;
     const uint32_t kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t l = p.kv_len[b];
     const uint32_t len = l > 0 ? min(uint32_t(l), p.max_len) : 0u, keep = min(len, p.budget);
@@ -74,10 +60,10 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
     int32_t* const kept = p.kept + row * p.budget;
     if (kvh == 0 && rank == 0 && tid == 0)
         p.count[b] = int32_t(keep);
-    for (uint32_t i = keep + rank * SNT + tid; i < p.budget; i += C * SNT)
+    for (uint32_t i = keep + rank * nt + tid; i < p.budget; i += C * nt)
         kept[i] = -1;
     if (len <= p.budget) {  // the same for the whole cluster
-        for (uint32_t i = rank * SNT + tid; i < len; i += C * SNT)
+        for (uint32_t i = rank * nt + tid; i < len; i += C * nt)
             kept[i] = int32_t(i);
         return;
     }
@@ -86,45 +72,76 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
     uint32_t want = p.budget - p.sinks - p.recent;     // how many of them stay
     const bool contest = want > 0;
     // warp g of the cluster owns rows [g * 32 * nk, (g + 1) * 32 * nk), lane i's every 32nd
-    const uint32_t nk = (len + C * SNT - 1) / (C * SNT), j0 = (rank * SWARPS + warp) * 32 * nk + lane;
+    const uint32_t nk = (len + C * nt - 1) / (C * nt), j0 = (rank * warps + warp) * 32 * nk + lane;
     uint32_t reg[REG ? SKEYS : 1];
     if (REG) {
 #pragma unroll
-        for (uint32_t i = 0; i < SKEYS; ++i)
-            if (i < nk)
-                reg[i] = j0 + i * 32 < len ? __float_as_uint(__ldg(w + j0 + i * 32)) : 0u;
-#pragma unroll
-        for (uint32_t i = 0; i < SKEYS; ++i)
-            if (i < nk)
-                reg[i] = weight_key(__uint_as_float(reg[i]));
+        for (uint32_t i = 0; i < SKEYS; ++i) {
+            if (i >= nk)
+                break;
+            reg[i] = j0 + i * 32 < len ? __float_as_uint(__ldg(w + j0 + i * 32)) : 0u;
+        }
     }
     // f(row, key) over this thread's rows, the whole warp in step
     auto each = [&](auto f) {
         if (REG) {
 #pragma unroll
-            for (uint32_t i = 0; i < SKEYS; ++i)
-                if (i < nk)
-                    f(j0 + i * 32, reg[REG ? i : 0]);
+            for (uint32_t i = 0; i < SKEYS; ++i) {
+                if (i >= nk)
+                    break;
+                f(j0 + i * 32, reg[REG ? i : 0]);
+            }
         } else {
-            for (uint32_t i = 0; i < nk; ++i)
-                f(j0 + i * 32, j0 + i * 32 < len ? weight_key(__ldg(w + j0 + i * 32)) : 0u);
+            for (uint32_t i = 0; i < nk; ++i) {
+                uint32_t key = j0 + i * 32 < len ? weight_key(__ldg(w + j0 + i * 32)) : 0u;
+                f(j0 + i * 32, key);
+            }
         }
     };
+    auto competes = [&](uint32_t j) { return j - lo < hi - lo; };  // lo <= j < hi
+    // REG: the rows that compete, and those kept in any case, as bits of this thread's keys.  The bits in which the
+    // warp's competing keys differ from one another, and all that any of them has.
+    uint32_t comp = 0, sure_bits = 0, ones = 0, zeros = 0, counted = 0, bit = 1;
+    each([&](uint32_t j, uint32_t& key) {
+        const bool c = competes(j);
+        if (REG) {
+            key = weight_key(__uint_as_float(key));
+            comp |= c ? bit : 0u;
+            sure_bits |= !c && j < len ? bit : 0u;
+            bit <<= 1;
+        } else {
+            counted += c ? 1u : 0u;
+        }
+        ones |= c ? key : 0u;
+        zeros |= c ? ~key : 0u;
+    });
+    if (REG)
+        counted = __popc(comp);
+    ones = __reduce_or_sync(0xffffffffu, ones);
+    const uint32_t differ = ones & __reduce_or_sync(0xffffffffu, zeros), warp_counted = __reduce_add_sync(0xffffffffu, counted);
     // T: the key of the last that stays, digit by digit; want: how many with key T stay
     uint32_t T = 0;
     for (uint32_t pass = 0; contest && pass < 3; ++pass) {
         const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        for (uint32_t i = tid; i < SBINS; i += SNT)
+        const uint32_t fixed = pass == 0 ? 0u : 0xFFFFFFFFu << (pass == 1 ? 21 : 10);  // the digits that are known
+        for (uint32_t i = tid; i < bins; i += nt)
             hist[i] = 0;
         __syncthreads();
-        each([&](uint32_t j, uint32_t key) {
-            const bool counts = j >= lo && j < hi && (pass == 0 || key >> (shift + (pass == 1 ? 11 : 10)) == T >> (shift + (pass == 1 ? 11 : 10)));
-            count_bin(hist, key >> shift & (bins - 1), counts);
-        });
+        if ((differ >> shift) == 0) {  // one digit, and one answer whether it counts, for the whole warp
+            if (lane == 0 && warp_counted && ((ones ^ T) & fixed) == 0)
+                atomicAdd(&hist[ones >> shift & (bins - 1)], warp_counted);
+        } else {
+            uint32_t m = comp;
+            each([&](uint32_t j, uint32_t& key) {
+                if ((REG ? (m & 1u) != 0 : competes(j)) && ((key ^ T) & fixed) == 0)
+                    atomicAdd(&hist[key >> shift & (bins - 1)], 1u);
+                m >>= 1;
+            });
+        }
         const uint32_t* all = hist;
         if (C > 1) {
             cluster.sync();
-            for (uint32_t i = tid; i < bins; i += SNT) {
+            for (uint32_t i = tid; i < bins; i += nt) {
                 uint32_t n = 0;
                 for (uint32_t c = 0; c < C; ++c)
                     n += cluster.map_shared_rank(hist, c)[i];
@@ -135,42 +152,66 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
         } else {
             __syncthreads();
         }
-        // the digit at which the count from the top reaches want: thread t looks at the bins - 1 - 2t th and the next
-        const uint32_t b0 = bins - 1 - 2 * tid, n0 = 2 * tid < bins ? all[b0] : 0u, n1 = 2 * tid < bins ? all[b0 - 1] : 0u;
-        const uint32_t incl = warp_incl_scan(n0 + n1);
-        if (lane == 31)
-            part[warp] = incl;
-        __syncthreads();
-        uint32_t above = incl - n0 - n1;
-        {
-            const uint32_t y = part[lane], z = warp_incl_scan(y) - y;
-            above += __shfl_sync(0xffffffffu, z, warp);
-        }
-        if (above < want && above + n0 + n1 >= want) {
-            const bool second = above + n0 < want;
-            found[0] = second ? b0 - 1 : b0;
-            found[1] = want - above - (second ? n0 : 0u);
+        // The digit at which the count from the top reaches want: 32 groups of bins are summed a warp a group (or
+        // several), then every warp finds the group and the digit in it for itself.
+        const uint32_t per = bins / 32;  // 64 or 32 bins a group, group 0 the highest
+        for (uint32_t g = warp; g < 32; g += warps) {
+            const uint32_t top = bins - 1 - g * per - lane;
+            const uint32_t n = __reduce_add_sync(0xffffffffu, all[top] + (per == 64 ? all[top - 32] : 0u));
+            if (lane == 0)
+                part[g] = n;
         }
         __syncthreads();
-        T |= found[0] << shift;
-        want = found[1];
+        uint32_t n = part[lane], above = warp_incl_scan(n) - n;
+        const int g = 31 - __clz(__ballot_sync(0xffffffffu, above < want));  // the last group not past it
+        above = __shfl_sync(0xffffffffu, above, g);
+        uint32_t bin = bins - 1 - g * per - lane;
+        n = all[bin];
+        uint32_t before = above + warp_incl_scan(n) - n;
+        uint32_t last = __shfl_sync(0xffffffffu, before + n, 31);
+        if (per == 64 && last < want) {
+            bin -= 32;
+            n = all[bin];
+            before = last + warp_incl_scan(n) - n;
+        }
+        const int d = 31 - __clz(__ballot_sync(0xffffffffu, before < want));
+        T |= __shfl_sync(0xffffffffu, bin, d) << shift;
+        want -= __shfl_sync(0xffffffffu, before, d);
+        __syncthreads();  // hist and part are written again
     }
     // kept rows without the ties, and ties, of this warp; then of those before it
-    uint32_t nk_sure = 0, n_tie = 0;
-    auto sure = [&](uint32_t j, uint32_t key) { return j < len && (j < lo || j >= hi || (contest && key > T)); };
-    auto tie = [&](uint32_t j, uint32_t key) { return contest && j >= lo && j < hi && key == T; };
-    each([&](uint32_t j, uint32_t key) {
-        nk_sure += __popc(__ballot_sync(0xffffffffu, sure(j, key)));
-        n_tie += __popc(__ballot_sync(0xffffffffu, tie(j, key)));
-    });
+    auto sure = [&](uint32_t j, uint32_t key) { return j < len && (!competes(j) || (contest && key > T)); };
+    auto tie = [&](uint32_t j, uint32_t key) { return contest && competes(j) && key == T; };
+    uint32_t n_sure = 0, n_tie = 0, tie_bits = 0;
+    if (contest || !REG) {
+        uint32_t m = comp;
+        bit = 1;
+        each([&](uint32_t j, uint32_t& key) {
+            if (REG) {
+                sure_bits |= (m & 1u) && key > T ? bit : 0u;
+                tie_bits |= (m & 1u) && key == T ? bit : 0u;
+                m >>= 1;
+                bit <<= 1;
+            } else {
+                n_sure += sure(j, key) ? 1u : 0u;
+                n_tie += tie(j, key) ? 1u : 0u;
+            }
+        });
+    }
+    if (REG) {
+        n_sure = __popc(sure_bits);
+        n_tie = __popc(tie_bits);
+    }
+    n_sure = __reduce_add_sync(0xffffffffu, n_sure);
+    n_tie = __reduce_add_sync(0xffffffffu, n_tie);
     if (lane == 0) {
-        ranks[0][warp] = nk_sure;
+        ranks[0][warp] = n_sure;
         ranks[1][warp] = n_tie;
     }
     __syncthreads();
     uint32_t at, ties;  // before this warp: kept rows without the ties, and ties
     {
-        const uint32_t a = ranks[0][lane], t = ranks[1][lane];
+        const uint32_t a = lane < warps ? ranks[0][lane] : 0u, t = lane < warps ? ranks[1][lane] : 0u;
         const uint32_t ai = warp_incl_scan(a), ti = warp_incl_scan(t);
         at = __shfl_sync(0xffffffffu, ai - a, warp);
         ties = __shfl_sync(0xffffffffu, ti - t, warp);
@@ -189,16 +230,41 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
     }
     at += min(ties, want);
     const uint32_t below = (1u << lane) - 1u;
-    each([&](uint32_t j, uint32_t key) {
-        const bool t = tie(j, key);
-        const uint32_t tied = __ballot_sync(0xffffffffu, t);
-        const bool stays = sure(j, key) || (t && ties + __popc(tied & below) < want);
-        const uint32_t stay = __ballot_sync(0xffffffffu, stays);
-        if (stays)
-            kept[at + __popc(stay & below)] = int32_t(j);
-        at += __popc(stay);
-        ties += __popc(tied);
-    });
+    if (n_sure == 0 && (n_tie == 0 || ties >= want))
+        return;
+    if (REG) {
+        // lane i takes the 32 rows of the warp's i-th keys
+        uint32_t stay = 0, tied = 0;
+        for (uint32_t i = 0; i < nk; ++i) {
+            const uint32_t a = __ballot_sync(0xffffffffu, sure_bits >> i & 1u);
+            stay = lane == i ? a : stay;
+        }
+        if (n_tie) {  // the same for the warp
+            for (uint32_t i = 0; i < nk; ++i) {
+                const uint32_t a = __ballot_sync(0xffffffffu, tie_bits >> i & 1u);
+                tied = lane == i ? a : tied;
+            }
+            const uint32_t n = __popc(tied), first = ties + warp_incl_scan(n) - n;
+            for (uint32_t room = first < want ? want - first : 0u, k = n; k > room; --k)
+                tied &= ~(0x80000000u >> __clz(tied));  // the highest go
+            stay |= tied;
+        }
+        const uint32_t n = __popc(stay);
+        at += warp_incl_scan(n) - n;
+        for (; stay; stay &= stay - 1)
+            kept[at++] = int32_t(j0 - lane + lane * 32 + __ffs(stay) - 1);
+    } else {
+        each([&](uint32_t j, uint32_t& key) {
+            const bool t = tie(j, key);
+            const uint32_t tied = __ballot_sync(0xffffffffu, t);
+            const bool stays = sure(j, key) || (t && ties + __popc(tied & below) < want);
+            const uint32_t stay = __ballot_sync(0xffffffffu, stays);
+            if (stays)
+                kept[at + __popc(stay & below)] = int32_t(j);
+            at += __popc(stay);
+            ties += __popc(tied);
+        });
+    }
 }
 
 // Out of place: a CTA copies CROWS rows of one kv head, 16 bytes a thread at a time, CU rows' loads in flight.
@@ -289,16 +355,15 @@ __global__ void __launch_bounds__(MNT) evict_in_place_kernel(const EvictParams p
 
 cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t st)
 {
-    // CTAs a row: enough that a thread's keys fit its registers (8 at most), and more, down to 8 keys a thread, while
-    // that leaves SMs idle.
-    const uint64_t rows = uint64_t(p.batch) * p.kv_heads;
+    // CTAs a row: as few as hold its keys in registers, 8 at most (see above for what a cluster costs).  Rows of up to
+    // 16 keys a thread of 256 take a small CTA, whose barriers are cheaper.
     uint32_t c = 1;
-    while (c < SMAX_CLUSTER && (uint64_t(c) * SNT * SKEYS < p.max_len ||
-                                (uint64_t(c) * SNT * 8 < p.max_len && 2 * c * rows <= p.num_sms)))
+    while (c < SMAX_CLUSTER && uint64_t(c) * SNT * SKEYS < p.max_len)
         c *= 2;
+    const uint32_t nt = p.max_len <= 256 * 16 ? 256 : SNT;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c, p.kv_heads, p.batch);
-    cfg.blockDim = dim3(SNT);
+    cfg.blockDim = dim3(nt);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;

@@ -149,7 +149,7 @@ struct EvictParams {
     int32_t* kept;     // [batch][kv_heads][budget]
     int32_t* new_len;  // [batch], may be kv_len
     int32_t* count;    // scratch [batch]: the rows each sequence keeps
-    uint32_t batch, max_len, kv_heads, dim, k_stride, out_stride, sinks, recent, budget, in_place, num_sms;
+    uint32_t batch, max_len, kv_heads, dim, k_stride, out_stride, sinks, recent, budget, in_place;
 };
 cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s);
 cudaError_t launch_cache_append(const AppendParams& p, int dtype, int dim, cudaStream_t s);

@@ -1127,7 +1127,6 @@ int mako_cache_evict(mako_attn_ctx* ctx, void* stream, int dtype, const void* k,
     p.recent = recent;
     p.budget = budget;
     p.in_place = same == 3;
-    p.num_sms = uint32_t(ctx->num_sms);
     ctx->launches += 2;
     auto st = static_cast<cudaStream_t>(stream);
     KernelTimer t(ctx, st);
