@@ -20,6 +20,10 @@
 //     hold anything; values of those tiles are cleaned in shared memory before the product: rows behind the draft become
 //     0, and so do single values that are not finite, which the rows that do see their token get back in the epilogue.
 //
+// The same kernel serves the decode that accumulates attention weights (DEC, mako_attention_decode_weights): one token a
+// sequence, its own key already counted in kv_len.  It stores the scores (4 bytes a key and head), and
+// weights_finish_kernel, once each row's maximum and sum are known, turns them into the keys' weights.
+//
 // Every wait is bounded (clock64); on a timeout the thread records a code in p.err, waits (bounded) for its own copies and
 // products in flight, and the CTA frees its TMEM and returns.
 #include "common.cuh"
@@ -36,8 +40,9 @@ constexpr long long WAIT_LIMIT = 1ll << 31;  // clock cycles (~1 s)
 // ahead of the epilogue that reads them.
 constexpr uint32_t BAD_RING = 8;
 
-template <int D, bool WIDE>
+template <int D, bool WIDE, bool DEC>
 struct TreeCfg {
+    static constexpr bool DECODE = DEC;
     static constexpr int STREAMS = D == 256 ? 1 : 2;
     static constexpr int NT = 128 + 128 * STREAMS;
     static constexpr uint32_t TK = D == 256 ? 64 : 128;         // keys a tile
@@ -65,7 +70,12 @@ struct __align__(64) TreeParams {
     const uint32_t* mask;
     int* err;
     uint64_t k_hstride;  // values a kv head of the cache
-    uint32_t batch, n_tok, heads, kv_heads, group, max_len, o_type, grid, min_units;
+    // DEC
+    float* scores;    // [batch][heads][s_stride] unscaled
+    float2* row_ml;   // [batch][heads]: (max in log2 units, sum) of rows written whole
+    float* weight;    // [batch][kv_heads][w_stride]
+    uint64_t s_stride, w_stride;
+    uint32_t batch, n_tok, heads, kv_heads, group, max_len, o_type, grid;
     float scale_log2;
 };
 
@@ -83,24 +93,27 @@ __device__ __forceinline__ uint32_t seq_drafted(const TreeParams& p, uint32_t b)
 }
 
 // The line of key tiles: sequence b holds kv_heads * rb segments (row blocks fastest) of `tiles` tiles each.
+// toks: the tokens that have rows; drafted: those that have a key behind the cached ones (none with DEC).
 struct SeqUnits {
-    uint32_t cached, drafted, tiles, rb;
+    uint32_t cached, drafted, toks, tiles, rb;
     __device__ uint32_t units(const TreeParams& p) const { return tiles * rb * p.kv_heads; }
 };
-template <uint32_t TK, uint32_t ROWS>
+template <class C>
 __device__ __forceinline__ SeqUnits seq_units(const TreeParams& p, uint32_t b)
 {
     SeqUnits s;
     s.cached = seq_cached(p, b);
-    s.drafted = seq_drafted(p, b);
-    s.tiles = (s.cached + s.drafted + TK - 1) / TK;
-    s.rb = (p.group * s.drafted + ROWS - 1) / ROWS;
+    s.drafted = C::DECODE ? 0u : seq_drafted(p, b);
+    s.toks = C::DECODE ? 1u : s.drafted;
+    s.tiles = (s.cached + s.drafted + C::TK - 1) / C::TK;
+    s.rb = (p.group * s.toks + C::ROWS - 1) / C::ROWS;
     return s;
 }
+// Down to one tile a CTA: 8 drafted tokens over 512 keys of 8 kv heads (40 tiles) run in 11.0 us so, 13.5 with two or
+// more tiles a CTA, 15.7 with four.
 __device__ __forceinline__ uint64_t units_per_cta(const TreeParams& p, uint64_t total)
 {
-    const uint64_t per = (total + p.grid - 1) / p.grid;
-    return per > p.min_units ? per : p.min_units;
+    return total ? (total + p.grid - 1) / p.grid : 1;
 }
 
 // One CTA's walk over its part of the line, segment piece by segment piece; every role walks alike.
@@ -111,14 +124,14 @@ struct Walk {
     bool first;      // the piece starts at the CTA's first unit
 };
 struct Piece {
-    uint32_t b, kvh, rblk, t0, nb, tiles, cached, drafted, slot;
+    uint32_t b, kvh, rblk, t0, nb, cached, drafted, rows, slot;  // rows: the segment line's (group * toks)
     bool whole;
 };
-template <uint32_t TK, uint32_t ROWS>
+template <class C>
 __device__ __forceinline__ bool next_piece(const TreeParams& p, Walk& w, Piece& x)
 {
     while (w.left && w.b < p.batch) {
-        const SeqUnits s = seq_units<TK, ROWS>(p, w.b);
+        const SeqUnits s = seq_units<C>(p, w.b);
         if (w.rem >= s.units(p)) {
             ++w.b;
             w.rem = 0;
@@ -130,7 +143,7 @@ __device__ __forceinline__ bool next_piece(const TreeParams& p, Walk& w, Piece& 
         x.rblk = seg % s.rb;
         x.t0 = w.rem % s.tiles;
         x.nb = min(s.tiles - x.t0, w.left);
-        x.tiles = s.tiles;
+        x.rows = p.group * s.toks;
         x.cached = s.cached;
         x.drafted = s.drafted;
         x.whole = x.nb == s.tiles;
@@ -199,10 +212,10 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u)
     return m;
 }
 
-template <int D, bool BF, bool WIDE>
-__global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(const __grid_constant__ TreeParams p)
+template <int D, bool BF, bool WIDE, bool DEC>
+__global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel(const __grid_constant__ TreeParams p)
 {
-    using C = TreeCfg<D, WIDE>;
+    using C = TreeCfg<D, WIDE, DEC>;
     constexpr uint32_t TK = C::TK, ROWS = C::ROWS, NS = C::NS, SC = TK;  // SC: TMEM columns of an S buffer
     constexpr uint32_t COLO = 256;
     extern __shared__ uint8_t smem_raw[];
@@ -246,9 +259,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
     }
     if (warp == 0) {
         // this CTA's part of the line: [u0, u1), then the sequence u0 lies in
-        uint64_t units = lane < p.batch ? seq_units<TK, ROWS>(p, lane).units(p) : 0, total = units;
+        uint64_t units = lane < p.batch ? seq_units<C>(p, lane).units(p) : 0, total = units;
         for (uint32_t i = lane + 32; i < p.batch; i += 32)
-            total += seq_units<TK, ROWS>(p, i).units(p);
+            total += seq_units<C>(p, i).units(p);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
             total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -271,7 +284,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                 break;
             }
             at += __shfl_sync(0xffffffffu, incl, 31);
-            units = i0 + 32 + lane < p.batch ? seq_units<TK, ROWS>(p, i0 + 32 + lane).units(p) : 0;
+            units = i0 + 32 + lane < p.batch ? seq_units<C>(p, i0 + 32 + lane).units(p) : 0;
         }
         if (lane == 0) {
             plan[0] = b;
@@ -296,7 +309,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
             tma_prefetch_desc(&p.tk);
             tma_prefetch_desc(&p.tv);
             uint32_t loads = 0;
-            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+            while (ok && next_piece<C>(p, w, x)) {
                 const int hd = int(x.b * p.kv_heads + x.kvh);
                 // loads in ring order
                 for (uint32_t i = 0; i < 2 * x.nb; ++i) {
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
             uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
             auto wait_full = [&](uint32_t n) { return mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
             auto wait_v = [&](uint32_t t) { return wait_full(n0 + v_at<WIDE>(t, x.nb)); };
-            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+            while (ok && next_piece<C>(p, w, x)) {
                 if (!(ok = mbar_wait(q_full, pieces & 1, WAIT_LIMIT)))
                     break;
                 ++pieces;
@@ -423,8 +436,13 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                         fence_after();
                         pv(y, C::STREAMS == 2 ? y : 0, vs, t, C::STREAMS == 2 ? t > 1 : t > 0);
                         umma_commit(empty(vs));
-                        if (C::STREAMS == 1 || t + 2 >= x.nb)
-                            umma_commit(pv_done(C::STREAMS == 2 ? y : 0));
+                        if (C::STREAMS == 1) {
+                            umma_commit(pv_done(0));  // every product, for a rescale of O
+                            if (t + 1 == x.nb)
+                                umma_commit(pv_done(1));  // the piece's last
+                        } else if (t + 2 >= x.nb) {
+                            umma_commit(pv_done(y));
+                        }
                         if (t + 2 < x.nb) {
                             const uint32_t kn = n0 + k_at<WIDE>(t + 2);
                             if (!(ok = wait_full(kn)))
@@ -448,11 +466,11 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
             // Rows past the drafted ones keep what the tile held: they only make rows of S and O that nobody reads.
             constexpr uint32_t CH = D / 8, RPI = 2 * (32 / CH);  // 16-byte chunks a row, rows the warps load at once
             uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
-            while (ok && next_piece<TK, ROWS>(p, w, x)) {
+            while (ok && next_piece<C>(p, w, x)) {
                 if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
                     break;
                 {
-                    const uint32_t rows = min(ROWS, p.group * x.drafted - x.rblk * ROWS), c = lane % CH;
+                    const uint32_t rows = min(ROWS, x.rows - x.rblk * ROWS), c = lane % CH;
                     uint32_t r = (warp - 2) * (RPI / 2) + lane / CH;
                     uint32_t tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
                     const uint16_t* src = static_cast<const uint16_t*>(p.q) +
@@ -519,12 +537,13 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
         const uint32_t y = (warp - 4) >> 2, ql = (warp & 3) * 32, row = ql + lane;
         const uint32_t tl = tmem + (ql << 16);
         const float scale = p.scale_log2;
-        uint32_t pieces = 0, sc = 0, pvn = 0;  // sc: parity of each s_full's phases, pvn: pv_done's phases so far
-        while (ok && next_piece<TK, ROWS>(p, w, x)) {
-            const uint32_t live_rows = p.group * x.drafted;
+        // sc: parity of each s_full's phases; pieces ended with tiles of this stream; tiles of all pieces so far
+        uint32_t pieces = 0, sc = 0, ends = 0, products = 0;
+        while (ok && next_piece<C>(p, w, x)) {
+            const uint32_t live_rows = x.rows;
             const uint32_t rbase = x.rblk * ROWS + (WIDE ? y * 128 : 0), r = rbase + row;
             const bool live = r < live_rows, warp_live = rbase + ql < live_rows;
-            const uint32_t tok = min(r, live_rows - 1) / p.group;
+            const uint32_t tok = DEC ? 0u : min(r, live_rows - 1) / p.group;
             float m = -INFINITY, l = 0.0f;
             uint32_t mine = 0;  // tiles of this stream so far
             const uint32_t step = WIDE || C::STREAMS == 1 ? 1 : 2;
@@ -535,8 +554,8 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                     break;
                 sc ^= 1u << sb;
                 fence_after();
+                uint32_t s[TK / 32][32];
                 if (warp_live) {
-                    uint32_t s[TK / 32][32];
                     if constexpr (TK == 128)
                         tmem_ld128(tl + sb * SC, s);
                     else
@@ -609,7 +628,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                     // with this S.  One stream: wait for it here.
                     if (__any_sync(0xffffffffu, resc && mine > 0)) {
                         if (C::STREAMS == 1)
-                            ok = __all_sync(0xffffffffu, mbar_wait(pv_done(0), (pvn + mine - 1) & 1, WAIT_LIMIT));
+                            ok = __all_sync(0xffffffffu, mbar_wait(pv_done(0), (products + mine - 1) & 1, WAIT_LIMIT));
                         fence_after();
                         const float gsc = resc ? f : 1.0f;
 #pragma unroll
@@ -630,16 +649,26 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                 mbar_arrive(p_full(sb));
                 if (!ok)
                     break;
+                if (DEC && live) {  // the row's scores, while the product runs; s_stride is a multiple of the tile
+                    float* const d =
+                        p.scores + (uint64_t(x.b) * p.heads + x.kvh * p.group + r) * p.s_stride + (x.t0 + t) * TK;
+#pragma unroll
+                    for (uint32_t c = 0; c < TK / 32; ++c)
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; e += 8) {
+                            const uint32_t u[8] = {s[c][e],     s[c][e + 1], s[c][e + 2], s[c][e + 3],
+                                                   s[c][e + 4], s[c][e + 5], s[c][e + 6], s[c][e + 7]};
+                            st_global_v8(d + c * 32 + e, u);
+                        }
+                }
             }
-            // the stream's last product (one stream: every product commits pv_done)
+            // The stream's last product.  One stream: on a barrier of its own, since pv_done(0) may by now have completed
+            // one phase or two since S was seen, which a wait by parity cannot tell apart.
             if (ok && mine > 0) {
-                const uint32_t ph = C::STREAMS == 1 ? pvn + x.nb - 1 : pvn;
-                // one stream: the last S was committed with the product two tiles before, so two phases may be due
-                if (C::STREAMS == 1 && x.nb > 1)
-                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done(0), (ph - 1) & 1, WAIT_LIMIT));
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(pv_done(C::STREAMS == 2 ? y : 0), ph & 1, WAIT_LIMIT));
+                ok = __all_sync(0xffffffffu, mbar_wait(pv_done(C::STREAMS == 2 ? y : 1), ends & 1, WAIT_LIMIT));
                 fence_after();
-                pvn += C::STREAMS == 1 ? x.nb : 1;
+                ++ends;
+                products += x.nb;
             }
             // ---- epilogue: the rows' o, or their part of it
             const uint32_t* const mybad = bad + pieces % BAD_RING * 8;
@@ -668,8 +697,12 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
                 const uint64_t doff =
                     x.whole ? ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + r % p.group) * D
                             : (uint64_t(x.slot) * ROWS + lrow) * D;
-                if (!x.whole && live && (!MERGE || y == 0))
-                    p.ml_part[uint64_t(x.slot) * ROWS + lrow] = make_float2(m, l);
+                if (live && (!MERGE || y == 0)) {
+                    if (!x.whole)
+                        p.ml_part[uint64_t(x.slot) * ROWS + lrow] = make_float2(m, l);
+                    else if (DEC)
+                        p.row_ml[uint64_t(x.b) * p.heads + x.kvh * p.group + r] = make_float2(m, l);
+                }
                 uint32_t any_bad = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -736,20 +769,22 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE>::NT), 1) tree_tc_kernel(cons
     }
 }
 
-// A warp a row: merges the pieces of a segment that several CTAs worked on; rows of segments written whole have
-// nothing to do.  Which pieces there are follows from the lengths alone and is worked out before the wait for the main
-// kernel; the weights of 32 pieces are made at once, a lane a piece, and their rows' loads do not depend on one another.
-constexpr uint32_t CMB_WARPS = 8;
-template <int D, bool WIDE>
-__global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p)
+// Where row r of (sequence b, kv head kvh) was worked on: CTAs c0 .. c1, in the rows `lrow` of their slots.
+struct RowPieces {
+    uint32_t c0, c1, slot0, lrow;
+    template <class C>
+    __device__ uint64_t at(uint32_t c) const
+    {
+        return uint64_t(c == c0 ? slot0 : 2 * c) * C::ROWS + lrow;
+    }
+};
+// Warp-collective.
+template <class C>
+__device__ __forceinline__ void line_sums(const TreeParams& p, uint32_t b, uint64_t& before, uint64_t& total)
 {
-    using C = TreeCfg<D, WIDE>;
-    constexpr uint32_t V = D / 32;
-    const uint32_t lane = threadIdx.x & 31, b = blockIdx.y, per_kv = p.group * p.n_tok;
-    const uint32_t i = blockIdx.x * CMB_WARPS + (threadIdx.x >> 5);
-    uint64_t before = 0, total = 0;
-    for (uint32_t k = lane; k < p.batch; k += 32) {
-        const uint64_t n = seq_units<C::TK, C::ROWS>(p, k).units(p);
+    before = total = 0;
+    for (uint32_t k = threadIdx.x & 31; k < p.batch; k += 32) {
+        const uint64_t n = seq_units<C>(p, k).units(p);
         total += n;
         before += k < b ? n : 0;
     }
@@ -758,44 +793,61 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __gr
         total += __shfl_xor_sync(0xffffffffu, total, o);
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    const SeqUnits s = seq_units<C::TK, C::ROWS>(p, b);
-    const uint32_t kvh = i / per_kv, r = i % per_kv;
-    if (kvh >= p.kv_heads || r >= p.group * s.drafted)
-        return;
-    const uint64_t per = units_per_cta(p, total);
+}
+template <class C>
+__device__ __forceinline__ RowPieces row_pieces(const SeqUnits& s, uint32_t kvh, uint32_t r, uint64_t before, uint64_t per)
+{
     const uint64_t u0 = before + uint64_t(kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
-    const uint32_t c0 = uint32_t(u0 / per), c1 = uint32_t((u1 - 1) / per);
-    if (c0 == c1)
-        return;
-    const uint32_t lrow = r % C::ROWS, slot0 = 2 * c0 + (u0 % per ? 1 : 0);
-    auto at = [&](uint32_t c) { return uint64_t(c == c0 ? slot0 : 2 * c) * C::ROWS + lrow; };
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    RowPieces x;
+    x.c0 = uint32_t(u0 / per);
+    x.c1 = uint32_t((u1 - 1) / per);
+    x.slot0 = 2 * x.c0 + (u0 % per ? 1 : 0);
+    x.lrow = r % C::ROWS;
+    return x;
+}
+// Merges 32 pieces' (max, sum), a lane a piece, into the running M and l; returns this piece's weight, f0 that of what
+// was merged before.  Warp-collective.
+__device__ __forceinline__ float merge_ml(float2 ml, float& M, float& l, float& f0)
+{
+    float m1 = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+    const float Mn = fmaxf(M, m1);
+    f0 = M == -INFINITY ? 0.0f : ex2(M - Mn);
+    M = Mn;
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+    float ls = ml.y * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        ls += __shfl_xor_sync(0xffffffffu, ls, o);
+    l = l * f0 + ls;
+    return f;
+}
+// Merges the pieces of one row into o (values at o0 on): WARPS warps of the CTA take every WARPS-th group of pieces and
+// meet in shared memory.  parts: WARPS * (D + 2) floats.
+template <int D, class C, uint32_t WARPS>
+__device__ __forceinline__ void combine_row(const TreeParams& p, const RowPieces& x, uint64_t o0, float* parts)
+{
+    constexpr uint32_t V = D / 32;
+    const uint32_t lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+    const uint32_t step = WARPS == 1 ? 32 : min(32u, (x.c1 - x.c0) / WARPS + 1);  // pieces a warp takes at once
     float M = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (uint32_t e = 0; e < V; ++e)
         acc[e] = 0.0f;
-    for (uint32_t cb = c0; cb <= c1; cb += 32) {
-        const uint32_t n = min(32u, c1 - cb + 1);
-        const float2 ml = lane < n ? p.ml_part[at(cb + lane)] : make_float2(-INFINITY, 0.0f);
-        float m1 = ml.x;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-        const float Mn = fmaxf(M, m1), f0 = M == -INFINITY ? 0.0f : ex2(M - Mn);
-        M = Mn;
-        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        float ls = ml.y * f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            ls += __shfl_xor_sync(0xffffffffu, ls, o);
-        l = l * f0 + ls;
+    for (uint32_t cb = x.c0 + warp * step; cb <= x.c1; cb += WARPS * step) {
+        const uint32_t n = min(step, x.c1 - cb + 1);
+        float f0;
+        const float f =
+            merge_ml(lane < n ? p.ml_part[x.at<C>(cb + lane)] : make_float2(-INFINITY, 0.0f), M, l, f0);
 #pragma unroll
         for (uint32_t e = 0; e < V; ++e)
             acc[e] *= f0;
 #pragma unroll 4
         for (uint32_t k = 0; k < n; ++k) {
             const float w = __shfl_sync(0xffffffffu, f, k);
-            const float* src = p.o_part + at(cb + k) * D + lane * V;
+            const float* src = p.o_part + x.at<C>(cb + k) * D + lane * V;
 #pragma unroll
             for (uint32_t e = 0; e < V; e += 2) {
                 const float2 z = __ldcs(reinterpret_cast<const float2*>(src + e));
@@ -804,17 +856,164 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __gr
             }
         }
     }
+    if (WARPS > 1) {
+        float* const mine = parts + warp * (D + 2);
+        if (lane == 0) {
+            mine[D] = M;
+            mine[D + 1] = l;
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < V; ++e)
+            mine[lane * V + e] = acc[e];
+        __syncthreads();
+        M = -INFINITY;
+#pragma unroll
+        for (uint32_t k = 0; k < WARPS; ++k)
+            M = fmaxf(M, parts[k * (D + 2) + D]);
+        for (uint32_t d = threadIdx.x; d < D; d += WARPS * 32) {
+            float o = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (uint32_t k = 0; k < WARPS; ++k) {
+                const float* const z = parts + k * (D + 2);
+                const float f = z[D] == -INFINITY ? 0.0f : ex2(z[D] - M);
+                o = fmaf(z[d], f, o);
+                sum = fmaf(z[D + 1], f, sum);
+            }
+            out_store1(p.o, o0 + d, sum != 0.0f ? o / sum : 0.0f, p.o_type);
+        }
+        return;
+    }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    const uint64_t o = ((uint64_t(b) * p.n_tok + r / p.group) * p.heads + kvh * p.group + r % p.group) * D + lane * V;
 #pragma unroll
     for (uint32_t e = 0; e < V; e += 2)
-        out_store2(p.o, o + e, acc[e] * inv, acc[e + 1] * inv, p.o_type);
+        out_store2(p.o, o0 + lane * V + e, acc[e] * inv, acc[e + 1] * inv, p.o_type);
 }
 
+// A warp a row: merges the pieces of a segment that several CTAs worked on; rows of segments written whole have
+// nothing to do.  Which pieces there are follows from the lengths alone and is worked out before the wait for the main
+// kernel; the weights of 32 pieces are made at once, a lane a piece, and their rows' loads do not depend on one another.
+constexpr uint32_t CMB_WARPS = 8;
 template <int D, bool WIDE>
+__global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p)
+{
+    using C = TreeCfg<D, WIDE, false>;
+    const uint32_t b = blockIdx.y, per_kv = p.group * p.n_tok, i = blockIdx.x * CMB_WARPS + (threadIdx.x >> 5);
+    uint64_t before, total;
+    line_sums<C>(p, b, before, total);
+    const SeqUnits s = seq_units<C>(p, b);
+    const uint32_t kvh = i / per_kv, r = i % per_kv;
+    RowPieces x{};
+    if (kvh < p.kv_heads && r < p.group * s.drafted)
+        x = row_pieces<C>(s, kvh, r, before, units_per_cta(p, total));
+    // Every CTA waits, with rows or without: what comes next in the stream waits for this kernel alone.
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    if (x.c0 == x.c1)
+        return;
+    combine_row<D, C, 1>(p, x, ((uint64_t(b) * p.n_tok + r / p.group) * p.heads + kvh * p.group + r % p.group) * D, nullptr);
+}
+
+// The second half of the decode with weights, for one kv head of a sequence.  CTAs below n_weight take WKEYS keys each:
+// a warp a head finds the row's maximum and sum, then each thread sums 2^(s * scale - max) / sum over the group's heads,
+// in their order, for four keys and adds that to their weights.  The others combine cut rows, one each, and write the zero
+// rows of empty sequences.
+constexpr uint32_t WNT = 256, WKEYS = 4 * WNT, WHEADS = 64;
+template <int D>
+__global__ void __launch_bounds__(WNT) weights_finish_kernel(const __grid_constant__ TreeParams p, uint32_t n_weight)
+{
+    using C = TreeCfg<D, false, true>;
+    __shared__ float2 ml[WHEADS];  // (max, 1 / sum) of up to WHEADS heads at a time
+    __shared__ float parts[WNT / 32 * (D + 2)];
+    const uint32_t b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t before, total;
+    line_sums<C>(p, b, before, total);
+    const SeqUnits s = seq_units<C>(p, b);
+    const uint64_t per = units_per_cta(p, total);
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");  // every CTA, as above
+    if (blockIdx.x >= n_weight) {
+        const uint32_t r = blockIdx.x - n_weight;
+        const uint64_t o0 = (uint64_t(b) * p.heads + kvh * p.group + r) * D;
+        if (s.tiles == 0) {
+            if (threadIdx.x < D)
+                out_store1(p.o, o0 + threadIdx.x, 0.0f, p.o_type);
+            return;
+        }
+        const RowPieces x = row_pieces<C>(s, kvh, r, before, per);
+        if (x.c0 == x.c1)
+            return;
+        combine_row<D, C, WNT / 32>(p, x, o0, parts);
+        return;
+    }
+    const uint32_t L = s.cached, j = blockIdx.x * WKEYS + threadIdx.x * 4;
+    if (blockIdx.x * WKEYS >= L)
+        return;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t h0 = 0; h0 < p.group; h0 += WHEADS) {
+        const uint32_t nh = min(WHEADS, p.group - h0);
+        const uint64_t row0 = uint64_t(b) * p.heads + kvh * p.group + h0;
+        __syncthreads();
+        for (uint32_t h = warp; h < nh; h += WNT / 32) {
+            const RowPieces x = row_pieces<C>(s, kvh, h0 + h, before, per);
+            float M = -INFINITY, l = 0.0f, f0;
+            if (x.c0 == x.c1) {
+                const float2 v = p.row_ml[row0 + h];
+                M = v.x;
+                l = v.y;
+            } else {
+                for (uint32_t cb = x.c0; cb <= x.c1; cb += 32)
+                    merge_ml(lane < x.c1 - cb + 1 ? p.ml_part[x.at<C>(cb + lane)] : make_float2(-INFINITY, 0.0f), M, l, f0);
+            }
+            if (lane == 0)
+                ml[h] = M == -INFINITY ? make_float2(0.0f, l) : make_float2(M, 1.0f / l);  // no maximum: l is 0 or NaN
+        }
+        __syncthreads();
+        if (j < L) {
+            const float* sc = p.scores + row0 * p.s_stride + j;
+            for (uint32_t h = 0; h < nh; ++h, sc += p.s_stride) {
+                const float4 z = __ldcs(reinterpret_cast<const float4*>(sc));
+                const float2 c = ml[h];
+                acc[0] += ex2(fmaf(z.x, p.scale_log2, -c.x)) * c.y;
+                acc[1] += ex2(fmaf(z.y, p.scale_log2, -c.x)) * c.y;
+                acc[2] += ex2(fmaf(z.z, p.scale_log2, -c.x)) * c.y;
+                acc[3] += ex2(fmaf(z.w, p.scale_log2, -c.x)) * c.y;
+            }
+        }
+    }
+    float* w = p.weight + (uint64_t(b) * p.kv_heads + kvh) * p.w_stride + j;
+    if (j + 4 <= L && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+        float4 z = *reinterpret_cast<float4*>(w);
+        z.x += acc[0];
+        z.y += acc[1];
+        z.z += acc[2];
+        z.w += acc[3];
+        *reinterpret_cast<float4*>(w) = z;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < L)
+            w[e] += acc[e];
+}
+
+// The dependent second kernel: scheduled while the main kernel runs out.
+template <typename... A>
+cudaError_t launch_dependent(void (*kern)(A...), dim3 grid, uint32_t threads, cudaStream_t st, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <int D, bool WIDE, bool DEC>
 cudaError_t launch_tree_t(const TreeArgs& a, bool bf, int* err, cudaStream_t st)
 {
-    using C = TreeCfg<D, WIDE>;
+    using C = TreeCfg<D, WIDE, DEC>;
     TreeParams p;
     if (!tile_map(&p.tk, a.k, bf, D, a.k_stride, a.batch * a.kv_heads, C::TK) ||
         !tile_map(&p.tv, a.v, bf, D, a.k_stride, a.batch * a.kv_heads, C::TK))
@@ -829,6 +1028,11 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool bf, int* err, cudaStream_t st)
     p.mask = a.mask;
     p.err = err;
     p.k_hstride = uint64_t(a.k_stride) * D;
+    p.scores = a.scores;
+    p.row_ml = a.row_ml;
+    p.weight = a.weight;
+    p.s_stride = a.s_stride;
+    p.w_stride = a.k_stride;
     p.batch = a.batch;
     p.n_tok = a.n_tok;
     p.heads = a.heads;
@@ -837,25 +1041,23 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool bf, int* err, cudaStream_t st)
     p.max_len = a.max_len;
     p.o_type = a.o_type;
     p.grid = a.ctas;
-    p.min_units = 2;
     p.scale_log2 = a.scale * kLog2e;
-    auto kern = bf ? tree_tc_kernel<D, true, WIDE> : tree_tc_kernel<D, false, WIDE>;
+    auto kern = bf ? tree_tc_kernel<D, true, WIDE, DEC> : tree_tc_kernel<D, false, WIDE, DEC>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess)
         return e;
     kern<<<a.ctas, C::NT, C::TOTAL, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess)
         return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((p.group * p.n_tok * p.kv_heads + CMB_WARPS - 1) / CMB_WARPS, p.batch);
-    cfg.blockDim = dim3(CMB_WARPS * 32);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tree_combine_kernel<D, WIDE>, p);
+    if constexpr (DEC) {
+        const uint32_t nw = (p.max_len + WKEYS - 1) / WKEYS, nc = p.group;
+        return launch_dependent<const TreeParams, uint32_t>(weights_finish_kernel<D>, dim3(nw + nc, p.kv_heads, p.batch),
+                                                            WNT, st, p, nw);
+    } else {
+        return launch_dependent<const TreeParams>(
+            tree_combine_kernel<D, WIDE>,
+            dim3((p.group * p.n_tok * p.kv_heads + CMB_WARPS - 1) / CMB_WARPS, p.batch), CMB_WARPS * 32, st, p);
+    }
 }
 
 } // namespace
@@ -868,11 +1070,26 @@ cudaError_t launch_tree(const TreeArgs& a, int dtype, int dim, int* err, cudaStr
     const bool bf = dtype == kBF16, wide = tree_rows(a.n_tok, a.heads / a.kv_heads, dim) == 256;
     switch (dim) {
     case 64:
-        return wide ? launch_tree_t<64, true>(a, bf, err, st) : launch_tree_t<64, false>(a, bf, err, st);
+        return wide ? launch_tree_t<64, true, false>(a, bf, err, st) : launch_tree_t<64, false, false>(a, bf, err, st);
     case 128:
-        return wide ? launch_tree_t<128, true>(a, bf, err, st) : launch_tree_t<128, false>(a, bf, err, st);
+        return wide ? launch_tree_t<128, true, false>(a, bf, err, st) : launch_tree_t<128, false, false>(a, bf, err, st);
     case 256:
-        return launch_tree_t<256, false>(a, bf, err, st);
+        return launch_tree_t<256, false, false>(a, bf, err, st);
+    default:
+        return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t launch_decode_weights(const TreeArgs& a, int dtype, int dim, int* err, cudaStream_t st)
+{
+    const bool bf = dtype == kBF16;
+    switch (dim) {
+    case 64:
+        return launch_tree_t<64, false, true>(a, bf, err, st);
+    case 128:
+        return launch_tree_t<128, false, true>(a, bf, err, st);
+    case 256:
+        return launch_tree_t<256, false, true>(a, bf, err, st);
     default:
         return cudaErrorInvalidValue;
     }

@@ -9,8 +9,6 @@
 // mma.sync (the group's q rows padded to 16), keeps its own running softmax and accumulator, and the warps merge at
 // the end into one partial (o unnormalised, max, sum) per (sequence, head, split); a sequence with one split writes
 // o directly.
-// With SCORES the same kernel also stores every scaled score, from which decode_weights_kernel makes the keys'
-// attention weights once the row's maximum and sum are known.
 // Kernel 2 (decode_combine_kernel): the log-sum-exp merge of a row's splits into o, launched as a programmatic
 // dependent of kernel 1 so that its launch overlaps kernel 1's last wave.
 #include "common.cuh"
@@ -36,14 +34,7 @@ __device__ __forceinline__ uint32_t seq_keys(const DecodeParams& p, uint32_t b)
     return l > 0 ? min(uint32_t(l), p.len) : 0u;
 }
 
-// A row's value: 0 for a row that sees no key; with SCORES a NaN sum stays NaN.
-template <bool SCORES>
-__device__ __forceinline__ float row_value(float o, float l)
-{
-    return (SCORES ? l != 0.0f : l > 0.0f) ? o / l : 0.0f;
-}
-
-template <int D, typename T, bool SCORES>
+template <int D, typename T>
 __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams p)
 {
     constexpr int ROWB = D * 2, CH = D / 8, KS = D / 16, TILE = DBN * ROWB;
@@ -133,16 +124,6 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
                 s[n][e] = x;
                 mx[e >> 1] = fmaxf(mx[e >> 1], x);
             }
-        if (SCORES) {
-            // rows of s_stride (a multiple of 64) scores, so that a tile's last pair lies within its row
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-                if (uint32_t(g + 8 * r) < nrows)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        *reinterpret_cast<float2*>(p.scores + (uint64_t(b) * p.heads + h0 + g + 8 * r) * p.s_stride + jb +
-                                                   n * 8 + 2 * tq) = make_float2(s[n][2 * r], s[n][2 * r + 1]);
-        }
         float f[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -165,8 +146,7 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float mm = m[e >> 1];
-                // (SCORES) a NaN score of a row with no maximum yet still makes its sum NaN
-                const float pe = mm == -INFINITY ? (SCORES && s[n][e] != s[n][e] ? s[n][e] : 0.0f) : ex2(s[n][e] - mm);
+                const float pe = mm == -INFINITY ? 0.0f : ex2(s[n][e] - mm);
                 s[n][e] = pe;
                 l[e >> 1] += pe;
             }
@@ -232,10 +212,8 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
             Ls += sm[(w * 2 + 1) * QR + r] * fw;
             O += so[(w * QR + r) * D + d] * fw;
         }
-        if (SCORES && d == 0 && ns == 1)
-            p.ml_part[(uint64_t(b) * p.heads + h0 + r) * p.n_splits] = make_float2(M, Ls);
         if (ns == 1 && !p.keep_partials) {
-            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + r) * D + d, row_value<SCORES>(O, Ls), p.o_type);
+            out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h0 + r) * D + d, Ls > 0.0f ? O / Ls : 0.0f, p.o_type);
         } else {
             const uint64_t row = (uint64_t(b) * p.heads + h0 + r) * p.n_splits + split;
             p.o_part[row * D + d] = O;
@@ -247,7 +225,7 @@ __global__ void __launch_bounds__(DNT, 2) decode_split_kernel(const DecodeParams
 
 // One CTA per (head, sequence), one thread per output value; the splits' weights 2^(m_s - M) go through shared
 // memory so each thread's loop is a stream of independent loads.
-template <int D, bool SCORES>
+template <int D>
 __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
 {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");  // kernel 1's writes are visible from here on
@@ -306,61 +284,7 @@ __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeParams p)
     for (; s < ns; ++s)
         acc[0] += src[uint64_t(s) * D] * w[s];
     const float O = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
-    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, row_value<SCORES>(O, tot), p.o_type);
-}
-
-// The keys' attention weights from the stored scores (SCORES): a CTA takes WKEYS keys of one kv head.  First a warp a
-// head merges the head's splits into its maximum and sum; then each thread sums 2^(s - max) / sum over the group's heads
-// for four keys, in the heads' order, and adds that to their weights.  Reads 4 bytes a (key, head), reads and writes 4 a
-// key.
-constexpr uint32_t WNT = 256, WKEYS = 4 * WNT, WHEADS = 64;
-__global__ void __launch_bounds__(WNT) decode_weights_kernel(const DecodeParams p)
-{
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    __shared__ float2 ml[WHEADS];  // (max, 1 / sum) of up to WHEADS heads at a time
-    const uint32_t b = blockIdx.z, kvh = blockIdx.y, group = p.heads / p.kv_heads;
-    const uint32_t L = seq_keys(p, b), j = blockIdx.x * WKEYS + threadIdx.x * 4;
-    if (blockIdx.x * WKEYS >= L)
-        return;
-    const uint32_t ns = min((L + p.chunk - 1) / p.chunk, p.n_splits);
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t h0 = 0; h0 < group; h0 += WHEADS) {
-        const uint32_t nh = min(WHEADS, group - h0);
-        __syncthreads();
-        for (uint32_t h = threadIdx.x / 32; h < nh; h += WNT / 32) {
-            const float2* src = p.ml_part + (uint64_t(b) * p.heads + kvh * group + h0 + h) * p.n_splits;
-            float M = -INFINITY, l = 0.0f;
-            for (uint32_t s = threadIdx.x % 32; s < ns; s += 32)
-                M = fmaxf(M, src[s].x);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            for (uint32_t s = threadIdx.x % 32; s < ns; s += 32)
-                l += src[s].x == -INFINITY ? 0.0f : src[s].y * ex2(src[s].x - M);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (threadIdx.x % 32 == 0)
-                ml[h] = M == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / l);
-        }
-        __syncthreads();
-        if (j < L) {
-            const float* s = p.scores + (uint64_t(b) * p.heads + kvh * group + h0) * p.s_stride + j;
-            for (uint32_t h = 0; h < nh; ++h, s += p.s_stride) {
-                const float4 x = *reinterpret_cast<const float4*>(s);
-                const float2 c = ml[h];
-                acc[0] += ex2(x.x - c.x) * c.y;
-                acc[1] += ex2(x.y - c.x) * c.y;
-                acc[2] += ex2(x.z - c.x) * c.y;
-                acc[3] += ex2(x.w - c.x) * c.y;
-            }
-        }
-    }
-    float* w = p.weight + (uint64_t(b) * p.kv_heads + kvh) * p.w_stride + j;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (j + e < L)
-            w[e] += acc[e];
+    out_store1(p.o, uint64_t(b) * p.o_bstride + uint64_t(h) * D + d, tot > 0.0f ? O / tot : 0.0f, p.o_type);
 }
 
 template <int D, typename T>
@@ -368,7 +292,7 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
     static_assert((4 * 2 * QR + 4 * QR * D) * 4 <= 2 * DST * DBN * D * 2, "merge buffer fits the stage ring");
-    auto kern = decode_split_kernel<D, T, false>;
+    auto kern = decode_split_kernel<D, T>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
@@ -385,14 +309,14 @@ cudaError_t launch_dec(const DecodeParams& p, cudaStream_t st)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, false>, p);
+    return cudaLaunchKernelEx(&cfg, decode_combine_kernel<D>, p);
 }
 
-template <int D, typename T, bool SCORES>
+template <int D, typename T>
 cudaError_t launch_split_only(const DecodeParams& p, cudaStream_t st)
 {
     constexpr int smem = (QR + 2 * DST * DBN) * D * 2;
-    auto kern = decode_split_kernel<D, T, SCORES>;
+    auto kern = decode_split_kernel<D, T>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
@@ -549,11 +473,11 @@ cudaError_t launch_decode_split(const DecodeParams& p, int dtype, int dim, cudaS
     const bool bf = dtype == kBF16;
     switch (dim) {
     case 64:
-        return bf ? launch_split_only<64, __nv_bfloat16, false>(p, st) : launch_split_only<64, __half, false>(p, st);
+        return bf ? launch_split_only<64, __nv_bfloat16>(p, st) : launch_split_only<64, __half>(p, st);
     case 128:
-        return bf ? launch_split_only<128, __nv_bfloat16, false>(p, st) : launch_split_only<128, __half, false>(p, st);
+        return bf ? launch_split_only<128, __nv_bfloat16>(p, st) : launch_split_only<128, __half>(p, st);
     case 256:
-        return bf ? launch_split_only<256, __nv_bfloat16, false>(p, st) : launch_split_only<256, __half, false>(p, st);
+        return bf ? launch_split_only<256, __nv_bfloat16>(p, st) : launch_split_only<256, __half>(p, st);
     default:
         return cudaErrorInvalidValue;
     }
@@ -574,54 +498,14 @@ cudaError_t launch_decode_combine(const DecodeParams& p, int dim, cudaStream_t s
     cfg.numAttrs = 1;
     switch (dim) {
     case 64:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64, false>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<64>, p);
     case 128:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128, false>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<128>, p);
     case 256:
-        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256, false>, p);
+        return cudaLaunchKernelEx(&cfg, decode_combine_kernel<256>, p);
     default:
         return cudaErrorInvalidValue;
     }
-}
-
-namespace {
-
-// A programmatic dependent of the stream's last kernel.
-cudaLaunchConfig_t dependent(dim3 grid, dim3 block, cudaStream_t st, cudaLaunchAttribute* attr)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = st;
-    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr->val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cfg;
-}
-
-template <int D>
-cudaError_t launch_weights_d(const DecodeParams& p, bool bf, cudaStream_t st)
-{
-    cudaError_t e = bf ? launch_split_only<D, __nv_bfloat16, true>(p, st) : launch_split_only<D, __half, true>(p, st);
-    if (e != cudaSuccess)
-        return e;
-    cudaLaunchAttribute attr;
-    auto cfg = dependent(dim3(p.heads, p.batch), dim3(D), st, &attr);
-    if ((e = cudaLaunchKernelEx(&cfg, decode_combine_kernel<D, true>, p)) != cudaSuccess || p.len == 0)
-        return e;
-    cfg = dependent(dim3((p.len + WKEYS - 1) / WKEYS, p.kv_heads, p.batch), dim3(WNT), st, &attr);
-    return cudaLaunchKernelEx(&cfg, decode_weights_kernel, p);
-}
-
-} // namespace
-
-cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t st)
-{
-    const bool bf = dtype == kBF16;
-    return dim == 64    ? launch_weights_d<64>(p, bf, st)
-           : dim == 128 ? launch_weights_d<128>(p, bf, st)
-                        : launch_weights_d<256>(p, bf, st);
 }
 
 cudaError_t launch_decode_xchg(const DecodeParams& p, const XchgParams& x, int dim, cudaStream_t st)

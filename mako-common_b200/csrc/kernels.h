@@ -73,10 +73,6 @@ struct DecodeParams {
     float scale;
     uint32_t keep_partials;  // 1: always write partials (the KV-sharded combine reads them), never o
     uint32_t o_type;         // element type of o: 0 fp32, 1 fp16, 2 bf16
-    // decode with weights: scores [batch][heads][s_stride] (scaled, log2 units), weight [batch][kv_heads][w_stride]
-    float* scores;
-    float* weight;
-    uint64_t s_stride, w_stride;
 };
 // Keys a split takes and how many splits, for the longest sequence max_len (chunk_opt: 0 automatic, else the
 // requested multiple of 64).
@@ -98,12 +94,16 @@ struct TreeArgs {
     const uint32_t* mask;   // [batch][n_tok][(n_tok + 31) / 32] or null: a chain
     uint32_t max_len, batch, n_tok, heads, kv_heads, k_stride, o_type, ctas;
     float scale;
+    // decode with weights (n_tok 1, n_new and mask null, kv_len counts every key)
+    float* scores;    // scratch [batch][heads][s_stride], s_stride a multiple of 128
+    float2* row_ml;   // scratch [batch][heads]
+    float* weight;    // [batch][kv_heads][k_stride]
+    uint64_t s_stride;
 };
 uint32_t tree_rows(uint32_t n_tok, uint32_t group, uint32_t dim);
 cudaError_t launch_tree(const TreeArgs& a, int dtype, int dim, int* err, cudaStream_t s);
-// Decode that also adds every key's attention weight to p.weight: splits, combine, weights.
-cudaError_t launch_decode_weights(const DecodeParams& p, int dtype, int dim, cudaStream_t s);
-
+// One token a sequence over its kv_len keys; every key's attention weight added to a.weight.
+cudaError_t launch_decode_weights(const TreeArgs& a, int dtype, int dim, int* err, cudaStream_t s);
 // Head-tile producers: y [heads][n_pad][dim] 16-bit, row row0 + r from x row map[r] (or r): head h's values at
 // x + row * ld + col0 + h * stride, RMS-normed times w when eps > 0, rotated when rope is 1 (halves i, i + rot / 2 over
 // the first rot values) or 2 (adjacent pairs over the whole head) by the (cos, sin) pairs cs + row * cs_row.

@@ -1035,44 +1035,46 @@ int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, c
         return MAKO_OK;
     if (!q || !k || !v || !o || !weight || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
         return fail(MAKO_EINVAL, "decode_weights: null or unaligned tensor (16-byte alignment)");
+    if (ctx->cc_major != 10)
+        return fail(MAKO_ENOTSUP, "decode_weights: the tcgen05 kernel needs sm_100 (sm_%d)", ctx->cc_major * 10);
     DeviceGuard dg(ctx->device);
     if (dg.err != cudaSuccess)
         return cuda_fail("set device", dg.err);
-    mako::DecodeParams p{};
-    p.q = q;
-    p.k = k;
-    p.v = v;
-    p.o = o;
-    p.kv_len = kv_len;
-    p.len = max_kv_len;
-    p.q_bstride = uint64_t(heads) * dim;
-    p.q_hstride = dim;
-    p.k_hstride = uint64_t(k_stride) * dim;
-    p.k_bstride = uint64_t(kv_heads) * p.k_hstride;
-    p.o_bstride = uint64_t(heads) * dim;
-    p.o_type = out_type(ctx, dtype);
-    p.batch = batch;
-    p.heads = heads;
-    p.kv_heads = kv_heads;
-    p.scale = 1.0f / sqrtf(float(dim));
-    mako::decode_plan(max_kv_len, batch, kv_heads, heads, ctx->num_sms, ctx->decode_chunk, &p.chunk, &p.n_splits);
-    p.weight = weight;
-    p.w_stride = k_stride;
-    p.s_stride = (uint64_t(max_kv_len) + 63) / 64 * 64;
-    void *op, *mlp, *sc;
-    if (int rc = scratch_kept(ctx, "dw_o", size_t(batch) * heads * p.n_splits * dim * 4, &op))
+    mako::TreeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.o = o;
+    a.kv_len = kv_len;
+    a.max_len = max_kv_len;
+    a.batch = batch;
+    a.n_tok = 1;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.k_stride = k_stride;
+    a.o_type = out_type(ctx, dtype);
+    a.ctas = ctx->persistent_ctas();
+    a.scale = 1.0f / sqrtf(float(dim));
+    a.weight = weight;
+    a.s_stride = (uint64_t(max_kv_len) + 127) / 128 * 128;
+    const size_t rows = size_t(2) * a.ctas * 128;
+    void *op, *mlp, *sc, *rml;
+    if (int rc = scratch_kept(ctx, "tree_o", rows * dim * 4, &op))
         return rc;
-    if (int rc = scratch_kept(ctx, "dw_ml", size_t(batch) * heads * p.n_splits * 8, &mlp))
+    if (int rc = scratch_kept(ctx, "tree_ml", rows * 8, &mlp))
         return rc;
-    if (int rc = scratch_kept(ctx, "dw_scores", size_t(batch) * heads * p.s_stride * 4, &sc))
+    if (int rc = scratch_kept(ctx, "dw_scores", size_t(batch) * heads * a.s_stride * 4, &sc))
         return rc;
-    p.o_part = static_cast<float*>(op);
-    p.ml_part = static_cast<float2*>(mlp);
-    p.scores = static_cast<float*>(sc);
-    ctx->launches += 3;
+    if (int rc = scratch_kept(ctx, "dw_ml", size_t(batch) * heads * 8, &rml))
+        return rc;
+    a.o_part = static_cast<float*>(op);
+    a.ml_part = static_cast<float2*>(mlp);
+    a.scores = static_cast<float*>(sc);
+    a.row_ml = static_cast<float2*>(rml);
+    ctx->launches += 2;
     auto st = static_cast<cudaStream_t>(stream);
     KernelTimer t(ctx, st);
-    cudaError_t e = mako::launch_decode_weights(p, dtype, int(dim), st);
+    cudaError_t e = mako::launch_decode_weights(a, dtype, int(dim), ctx->err, st);
     t.stop();
     return launched("decode_weights", e);
 }
