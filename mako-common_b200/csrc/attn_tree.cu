@@ -311,6 +311,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             uint32_t loads = 0;
             while (ok && next_piece<C>(p, w, x)) {
                 const int hd = int(x.b * p.kv_heads + x.kvh);
+                // Tiles that no other row block reads leave L2 first: the scores and parts stay (8 x 16-32K keys with
+                // weights 148 -> 141 us, one sequence of 131072 70 -> 62).
+                const uint64_t hint = x.rows <= ROWS ? l2_evict_first() : l2_evict_normal();
                 // loads in ring order
                 for (uint32_t i = 0; i < 2 * x.nb; ++i) {
                     bool is_k;
@@ -339,8 +342,8 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                     const uint32_t bar = !is_k && (x.t0 + t + 1) * TK > x.cached ? v_raw(s) : full(s);
                     mbar_expect_tx(bar, C::SLOT);
                     for (uint32_t c = 0; c < D / 64; ++c)
-                        tma_load_3d(sR + s * C::SLOT + c * C::KBOX, is_k ? &p.tk : &p.tv, bar, c * 64,
-                                    int((x.t0 + t) * TK), hd);
+                        tma_load_3d_hint(sR + s * C::SLOT + c * C::KBOX, is_k ? &p.tk : &p.tv, bar, c * 64,
+                                         int((x.t0 + t) * TK), hd, hint);
                     loads = n + 1;
                 }
                 n0 += 2 * x.nb;
