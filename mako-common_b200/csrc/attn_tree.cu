@@ -356,25 +356,35 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             }
         } else if (warp == 1 && lane == 0) {
             // ---------------- UMMA issuer ----------------
+            // Descriptors: one 64-bit add an operand (the start address field never carries into the next).
             constexpr uint32_t F = BF ? 1u : 0u;
             const uint32_t idesc_qk = idesc_f16(F, F, 0, 0, 128, TK);
             const uint32_t idesc_pv = idesc_f16(F, F, 0, 1, 128, D);
+            const uint64_t dq = sdesc(sQ, 16, 1024), dk = sdesc(sR, 16, 1024), dv = sdesc(sR, C::KBOX, 1024);
             auto qk = [&](uint32_t sbuf, uint32_t qt, uint32_t slot) {
+                const uint64_t a = dq + (qt * C::QTILE >> 4), b = dk + (slot * C::SLOT >> 4);
 #pragma unroll
                 for (uint32_t ks = 0; ks < D / 16; ++ks)
-                    umma_ss(tmem + sbuf * SC, sdesc(sQ + qt * C::QTILE + (ks >> 2) * C::QBOX + (ks & 3) * 32, 16, 1024),
-                            sdesc(sR + slot * C::SLOT + (ks >> 2) * C::KBOX + (ks & 3) * 32, 16, 1024), idesc_qk, ks > 0);
+                    umma_ss(tmem + sbuf * SC, a + (((ks >> 2) * C::QBOX + (ks & 3) * 32) >> 4),
+                            b + (((ks >> 2) * C::KBOX + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
             };
             // P.V over the tile's 16-key groups that hold keys (the cleaner has made the last group's other rows 0)
             auto pv = [&](uint32_t sbuf, uint32_t ot, uint32_t slot, uint32_t t, bool acc) {
-                const uint32_t groups = min(TK, x.cached + x.drafted - (x.t0 + t) * TK) + 15;
+                const uint64_t b = dv + (slot * C::SLOT >> 4);
+                const uint32_t keys = x.cached + x.drafted - (x.t0 + t) * TK, d = tmem + COLO + ot * 128, a = tmem + sbuf * SC;
+                if (keys >= TK) {
 #pragma unroll
-                for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
+                    for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
 #pragma unroll
-                    for (uint32_t kk = 0; kk < TK / 16; ++kk)
-                        if (kk < groups / 16)
-                            umma_ts(tmem + COLO + ot * 128, tmem + sbuf * SC + part * (TK / 2) + kk * 8,
-                                sdesc(sR + slot * C::SLOT + kk * 2048, C::KBOX, 1024), idesc_pv, acc || part > 0 || kk > 0);
+                        for (uint32_t kk = 0; kk < TK / 16; ++kk)
+                            umma_ts(d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
+                                    acc || part > 0 || kk > 0);
+                } else {
+                    for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
+                        for (uint32_t kk = 0; kk < (keys + 15) / 16; ++kk)
+                            umma_ts(d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
+                                    acc || part > 0 || kk > 0);
+                }
             };
             uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
             auto wait_full = [&](uint32_t n) { return mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
