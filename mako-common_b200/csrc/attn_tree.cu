@@ -58,6 +58,12 @@ struct TreeCfg {
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
+// mbar_wait for a whole warp in step.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, long long limit)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
+}
+
 struct __align__(64) TreeParams {
     CUtensorMap tk, tv;
     const void* q;
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
     uint32_t* const bad = reinterpret_cast<uint32_t*>(smem + C::BAD);
     float2* const xchg = reinterpret_cast<float2*>(smem + C::XCHG);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the combine may be scheduled now
     if (threadIdx.x == 32) {
         for (uint32_t s = 0; s < NS; ++s) {
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = plan[3];
+    const uint32_t tmem = __shfl_sync(0xffffffffu, plan[3], 0);
     Walk w{plan[0], plan[1], plan[2], true};
     Piece x;
     bool ok = true;
@@ -354,8 +360,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 for (uint32_t n = loads > NS ? loads - NS : 0; n < loads; ++n)
                     mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT);
             }
-        } else if (warp == 1 && lane == 0) {
-            // ---------------- UMMA issuer ----------------
+        } else if (warp == 1) {
+            // ---------------- UMMA issuer: the whole warp in step, one lane issues ----------------
+            const uint32_t lead = elect_lane();
             // Descriptors: one 64-bit add an operand (the start address field never carries into the next).
             constexpr uint32_t F = BF ? 1u : 0u;
             const uint32_t idesc_qk = idesc_f16(F, F, 0, 0, 128, TK);
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 const uint64_t a = dq + (qt * C::QTILE >> 4), b = dk + (slot * C::SLOT >> 4);
 #pragma unroll
                 for (uint32_t ks = 0; ks < D / 16; ++ks)
-                    umma_ss(tmem + sbuf * SC, a + (((ks >> 2) * C::QBOX + (ks & 3) * 32) >> 4),
+                    umma_ss_lead(lead, tmem + sbuf * SC, a + (((ks >> 2) * C::QBOX + (ks & 3) * 32) >> 4),
                             b + (((ks >> 2) * C::KBOX + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
             };
             // P.V over the tile's 16-key groups that hold keys (the cleaner has made the last group's other rows 0)
@@ -377,20 +384,24 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                     for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
 #pragma unroll
                         for (uint32_t kk = 0; kk < TK / 16; ++kk)
-                            umma_ts(d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
+                            umma_ts_lead(lead, d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
                                     acc || part > 0 || kk > 0);
                 } else {
                     for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
                         for (uint32_t kk = 0; kk < (keys + 15) / 16; ++kk)
-                            umma_ts(d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
+                            umma_ts_lead(lead, d, a + part * (TK / 2) + kk * 8, b + (kk * 2048 >> 4), idesc_pv,
                                     acc || part > 0 || kk > 0);
                 }
             };
             uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
-            auto wait_full = [&](uint32_t n) { return mbar_wait(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
+            auto wait_full = [&](uint32_t n) { return mbar_wait_warp(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
             auto wait_v = [&](uint32_t t) { return wait_full(n0 + v_at<WIDE>(t, x.nb)); };
             while (ok && next_piece<C>(p, w, x)) {
-                if (!(ok = mbar_wait(q_full, pieces & 1, WAIT_LIMIT)))
+                x.nb = __shfl_sync(0xffffffffu, x.nb, 0);  // so that the compiler knows it to be uniform
+                x.t0 = __shfl_sync(0xffffffffu, x.t0, 0);
+                x.cached = __shfl_sync(0xffffffffu, x.cached, 0);
+                x.drafted = __shfl_sync(0xffffffffu, x.drafted, 0);
+                if (!(ok = mbar_wait_warp(q_full, pieces & 1, WAIT_LIMIT)))
                     break;
                 ++pieces;
                 if (WIDE) {
@@ -399,34 +410,34 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                     fence_after();
                     for (uint32_t y = 0; y < 2; ++y) {
                         qk(y, y, n0 % NS);
-                        umma_commit(s_full(y));
+                        umma_commit_lead(lead, s_full(y));
                     }
-                    umma_commit(empty(n0 % NS));
+                    umma_commit_lead(lead, empty(n0 % NS));
                     if (x.nb == 1)
-                        umma_commit(q_empty);
+                        umma_commit_lead(lead, q_empty);
                     for (uint32_t t = 0; t < x.nb && ok; ++t) {
                         const uint32_t vs = (n0 + 2 * t + 1) % NS, ks = (n0 + 2 * t + 2) % NS;
                         ok = wait_v(t);
                         for (uint32_t y = 0; y < 2 && ok; ++y) {
-                            if (!(ok = mbar_wait(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
+                            if (!(ok = mbar_wait_warp(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
                                 break;
                             pc ^= 1u << y;
                             fence_after();
                             pv(y, y, vs, t, t > 0);
                             if (y == 1)
-                                umma_commit(empty(vs));
+                                umma_commit_lead(lead, empty(vs));
                             if (t + 1 < x.nb) {
                                 if (y == 0 && !(ok = wait_full(n0 + 2 * t + 2)))
                                     break;
                                 qk(y, y, ks);
-                                umma_commit(s_full(y));
+                                umma_commit_lead(lead, s_full(y));
                                 if (y == 1) {
-                                    umma_commit(empty(ks));
+                                    umma_commit_lead(lead, empty(ks));
                                     if (t + 2 == x.nb)
-                                        umma_commit(q_empty);
+                                        umma_commit_lead(lead, q_empty);
                                 }
                             } else {
-                                umma_commit(pv_done(y));
+                                umma_commit_lead(lead, pv_done(y));
                             }
                         }
                     }
@@ -436,44 +447,44 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                             break;
                         fence_after();
                         qk(t, 0, (n0 + t) % NS);
-                        umma_commit(s_full(t));
-                        umma_commit(empty((n0 + t) % NS));
+                        umma_commit_lead(lead, s_full(t));
+                        umma_commit_lead(lead, empty((n0 + t) % NS));
                         if (t + 1 == x.nb)
-                            umma_commit(q_empty);
+                            umma_commit_lead(lead, q_empty);
                     }
                     for (uint32_t t = 0; t < x.nb && ok; ++t) {
                         const uint32_t y = t & 1, vs = (n0 + v_at<WIDE>(t, x.nb)) % NS;
-                        if (!(ok = wait_v(t) && mbar_wait(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
+                        if (!(ok = wait_v(t) && mbar_wait_warp(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
                             break;
                         pc ^= 1u << y;
                         fence_after();
                         pv(y, C::STREAMS == 2 ? y : 0, vs, t, C::STREAMS == 2 ? t > 1 : t > 0);
-                        umma_commit(empty(vs));
+                        umma_commit_lead(lead, empty(vs));
                         if (C::STREAMS == 1) {
-                            umma_commit(pv_done(0));  // every product, for a rescale of O
+                            umma_commit_lead(lead, pv_done(0));  // every product, for a rescale of O
                             if (t + 1 == x.nb)
-                                umma_commit(pv_done(1));  // the piece's last
+                                umma_commit_lead(lead, pv_done(1));  // the piece's last
                         } else if (t + 2 >= x.nb) {
-                            umma_commit(pv_done(y));
+                            umma_commit_lead(lead, pv_done(y));
                         }
                         if (t + 2 < x.nb) {
                             const uint32_t kn = n0 + k_at<WIDE>(t + 2);
                             if (!(ok = wait_full(kn)))
                                 break;
                             qk(y, 0, kn % NS);
-                            umma_commit(s_full(y));
-                            umma_commit(empty(kn % NS));
+                            umma_commit_lead(lead, s_full(y));
+                            umma_commit_lead(lead, empty(kn % NS));
                             if (t + 3 == x.nb)
-                                umma_commit(q_empty);
+                                umma_commit_lead(lead, q_empty);
                         }
                     }
                 }
                 n0 += 2 * x.nb;
             }
-            if (!ok)
+            if (!ok && lane == 0)
                 atomicExch(p.err, 42);
-            umma_commit(mma_done);  // every product issued above has finished before TMEM is freed
-            mbar_wait(mma_done, 0, WAIT_LIMIT);
+            umma_commit_lead(lead, mma_done);  // every product issued above has finished before TMEM is freed
+            mbar_wait_warp(mma_done, 0, WAIT_LIMIT);
         } else if (warp >= 2) {
             // ---------------- q loaders, the second also cleans the drafted values ----------------
             // Rows past the drafted ones keep what the tile held: they only make rows of S and O that nobody reads.
