@@ -487,9 +487,11 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             mbar_wait_warp(mma_done, 0, WAIT_LIMIT);
         } else if (warp >= 2) {
             // ---------------- q loaders, the second also cleans the drafted values ----------------
-            // Rows past the drafted ones keep what the tile held: they only make rows of S and O that nobody reads.
+            // Rows past the drafted ones are zero: nobody reads what S and O hold for them, but products of zeros draw less
+            // power, which is what holds the clock down here.
             constexpr uint32_t CH = D / 8, RPI = 2 * (32 / CH);  // 16-byte chunks a row, rows the warps load at once
             uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
+            uint32_t dirty = ROWS;          // rows from here on are zero
             while (ok && next_piece<C>(p, w, x)) {
                 if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
                     break;
@@ -499,12 +501,14 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                     uint32_t tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
                     const uint16_t* src = static_cast<const uint16_t*>(p.q) +
                                           ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + g) * D + c * 8;
-                    for (; r < rows; r += RPI) {
-                        cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128), src, true);
+                    for (; r < max(rows, dirty); r += RPI) {
+                        cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128),
+                                   r < rows ? src : static_cast<const uint16_t*>(p.q), r < rows);
                         src += RPI * D;
                         for (g += RPI; g >= p.group; g -= p.group)
                             src += (p.heads - p.group) * D;  // the group's heads of the next token
                     }
+                    dirty = rows;
                     cp_async_commit();
                     cp_async_wait<0>();
                     fence_proxy_async_smem();

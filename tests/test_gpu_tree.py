@@ -174,6 +174,39 @@ def test_unseen_values_have_no_effect(ctx, dtype, dim, n_tok):
         assert torch.isnan(g[sees][:, :H // KV]).all()
 
 
+@pytest.mark.parametrize("dim,n_tok", [(64, 5), (128, 5), (128, 70), (256, 5)])
+def test_value_ranges(ctx, dim, n_tok):
+    """bf16 values far outside fp16's range and at its ends, alike in all keys and by groups of 32 keys, and zero."""
+    import cache_cases as C
+    import torch
+    H, KV, L = 4, 2, 500
+    q, k = C.randn(1, 1, n_tok, H, dim, dtype=1), C.randn(2, 1, KV, L + n_tok, dim, dtype=1)
+    v0 = C.randn(3, 1, KV, L + n_tok, dim, dtype=1)
+    see, mask = C.random_tree(4, 1, n_tok)
+    groups = torch.arange(L + n_tok, device="cuda")[:, None] // 32 % 4
+    mixed = torch.tensor([2.0 ** -40, 1.0, 2.0 ** 30, 2.0 ** -9], device="cuda")[groups]
+    for scale in (2.0 ** -60, 2.0 ** -11, 2.0 ** -9, 2.0 ** 13, 2.0 ** 14, 2.0 ** 60, 0.0, mixed):
+        v = (v0.float() * scale).to(torch.bfloat16)
+        o = torch.full((1, n_tok, H * dim), 3.0, device="cuda")
+        ctx.attention_tree(q, k, v, o, 1, n_tok, None, C.i32([L]), L, H, KV, dim, L + n_tok, mask)
+        want, tol = want_rows(q[0], k[0], v[0], L, n_tok, see[0], 1)
+        assert ((o[0].double() - want).abs() <= tol).all(), scale
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_seen_values_that_are_not_finite(ctx, dtype):
+    """A cached key's NaN value, seen by all, makes its column NaN in every row and no other."""
+    import cache_cases as C
+    import torch
+    n, H, KV, D, L = 5, 4, 2, 128, 300
+    q, k, v = C.randn(1, 1, n, H, D, dtype=dtype), C.randn(2, 1, KV, L + n, D, dtype=dtype), C.randn(3, 1, KV, L + n, D, dtype=dtype)
+    v[0, 1, 70, 9] = float("nan")
+    o = torch.zeros(1, n, H * D, device="cuda")
+    ctx.attention_tree(q, k, v, o, 1, n, None, C.i32([L]), L, H, KV, D, L + n)
+    bad = torch.isnan(o.view(n, H, D))
+    assert bad[:, 2:, 9].all() and bad.sum() == n * 2
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 def test_large_scores(ctx, dtype):
     """Scores in the thousands: one key takes almost all weight, the maximum moves from tile to tile."""
