@@ -58,10 +58,17 @@ struct TreeCfg {
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
-// mbar_wait for a whole warp in step.
+// mbar_wait for a whole warp in step, polling with a test that never suspends the warp: waking up from a suspended wait
+// cost the products' issuer up to half its time (16-token trees of bf16 142 -> 136 us, 64-wide heads 100 -> 82).
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, long long limit)
 {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
+    bool ok = mbar_test(bar, parity);
+    if (!ok) {
+        const long long t0 = clock64();
+        while (!(ok = mbar_test(bar, parity)) && clock64() - t0 < limit) {
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 
 struct __align__(64) TreeParams {

@@ -176,14 +176,14 @@ def test_unseen_values_have_no_effect(ctx, dtype, dim, n_tok):
 
 @pytest.mark.parametrize("dim,n_tok", [(64, 5), (128, 5), (128, 70), (256, 5)])
 def test_value_ranges(ctx, dim, n_tok):
-    """bf16 values far outside fp16's range and at its ends, alike in all keys and by groups of 32 keys, and zero."""
+    """bf16 values far outside fp16's range and at its ends, alike in all keys and by groups of 16 keys, and zero."""
     import cache_cases as C
     import torch
     H, KV, L = 4, 2, 500
     q, k = C.randn(1, 1, n_tok, H, dim, dtype=1), C.randn(2, 1, KV, L + n_tok, dim, dtype=1)
     v0 = C.randn(3, 1, KV, L + n_tok, dim, dtype=1)
     see, mask = C.random_tree(4, 1, n_tok)
-    groups = torch.arange(L + n_tok, device="cuda")[:, None] // 32 % 4
+    groups = torch.arange(L + n_tok, device="cuda")[:, None] // 16 % 4
     mixed = torch.tensor([2.0 ** -40, 1.0, 2.0 ** 30, 2.0 ** -9], device="cuda")[groups]
     for scale in (2.0 ** -60, 2.0 ** -11, 2.0 ** -9, 2.0 ** 13, 2.0 ** 14, 2.0 ** 60, 0.0, mixed):
         v = (v0.float() * scale).to(torch.bfloat16)
