@@ -217,10 +217,11 @@ int mako_proj(mako_attn_ctx* ctx, void* stream, int dtype, const void* w, const 
  * No reference counterpart: the reference keeps no cache across tokens beyond what attention() reads.  The cache is
  * the one mako_attention_decode reads: k and v [batch][kv_heads][k_stride][dim] of `dtype`, kv_len [batch] int32 on the
  * device, dim 64, 128 or 256; an entry of kv_len <= 0 is an empty sequence.  A step of speculative decoding appends
- * the drafted tokens (mako_cache_append), attends them (mako_attention_tree) and keeps the accepted ones; a bounded
- * cache decodes with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls
- * use is never freed before the context is destroyed, so a CUDA graph that captured one stays valid when a later, larger
- * call grows it. */
+ * the drafted tokens (mako_cache_append), attends them (mako_attention_tree) and raises kv_len by the accepted ones: of a
+ * chain they lie in place, of a tree the caller appends them again, in order, behind kv_len.  A bounded cache decodes
+ * with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls use is not
+ * freed before the context is destroyed, so a CUDA graph that captured one stays valid when a later, larger call grows
+ * it. */
 
 /* Rotation partners: value i of the rotated part with i + rot / 2, or 2i with 2i + 1. */
 enum { MAKO_ROPE_HALVES = 1, MAKO_ROPE_PAIRS = 2 };
@@ -254,14 +255,14 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
                       uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
                       const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride);
 
-/* Attention for a tree of drafted tokens over a cache: q [batch][n_tok][heads][dim] (n_tok at most 256), the drafted
- * tokens' keys and values at cache rows kv_len[b] + i as mako_cache_append leaves them.  Token i < n_new[b] (null: n_tok)
- * sees the cached keys [0, kv_len[b]) and the drafted keys j < n_new[b] with bit j % 32 of
+/* Attention for a tree of drafted tokens over a cache: q [batch][n_tok][heads][dim] (batch at most 65535, n_tok 256),
+ * the drafted tokens' keys and values at cache rows kv_len[b] + i as mako_cache_append leaves them.  Token i < n_new[b]
+ * (null: n_tok) sees the cached keys [0, kv_len[b]) and the drafted keys j < n_new[b] with bit j % 32 of
  * mask[b][i][j / 32] set (uint32 [batch][n_tok][(n_tok + 31) / 32]; null: j <= i, a chain); o [batch][n_tok][heads * dim]
  * floats (or 16-bit, MAKO_OPT_OUTPUT_16BIT), rows i >= n_new[b] left as they are, a row that sees nothing is 0.
  * A length above max_kv_len is read as max_kv_len; max_kv_len + n_tok is at most k_stride.  What cache rows hold that
  * no token of the sequence sees, NaN or infinities among it, has no effect, and neither has a drafted token on those
- * that do not see it. */
+ * that do not see it.  Equal calls give equal results.  sm_100 only (MAKO_ENOTSUP otherwise). */
 int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
                         float* o, uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len,
                         uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t k_stride,
@@ -269,7 +270,8 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
 
 /* mako_attention_decode that also accumulates every key's attention weight: weight [batch][kv_heads][k_stride] fp32
  * receives, at key j < kv_len[b], the sum over the kv head's query heads of softmax_j added to what it held; entries at
- * or past the length are left as they are.  The order of every sum is fixed: equal calls give equal results. */
+ * or past the length are left as they are.  The order of every sum is fixed: equal calls give equal results.
+ * batch and kv_heads at most 65535; sm_100 only (MAKO_ENOTSUP otherwise). */
 int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
                                   const void* v, float* o, float* weight, uint32_t batch, const int32_t* kv_len,
                                   uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim,
@@ -283,7 +285,7 @@ int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, c
  * number), new_len [batch] int32 min(kv_len, budget).  A sequence within the budget keeps all its rows.  Other rows of the
  * outputs are left as they are.  In place: k_out == k, v_out == v, weight_out == weight and out_stride == k_stride;
  * otherwise the outputs share no memory with the inputs (checked for equal addresses), except that new_len may be kv_len.
- * budget <= out_stride; a length above max_kv_len (<= k_stride) is read as max_kv_len. */
+ * budget <= out_stride; a length above max_kv_len (<= k_stride) is read as max_kv_len; batch and kv_heads at most 65535. */
 int mako_cache_evict(mako_attn_ctx* ctx, void* stream, int dtype, const void* k, const void* v, const float* weight,
                      uint32_t batch, const int32_t* kv_len, uint32_t max_kv_len, uint32_t kv_heads, uint32_t dim,
                      uint32_t k_stride, uint32_t sinks, uint32_t recent, uint32_t budget, void* k_out, void* v_out,

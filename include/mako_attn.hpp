@@ -96,6 +96,42 @@ public:
     {
         check(mako_heads_clear(ctx_, stream_, dtype_, y, dim, n_pad, from, heads));
     }
+    // ---- operators around a KV cache (no reference members): k, v [batch][kv_heads][k_stride][dim], kv_len [batch]
+    // Projected tokens into the cache, q and k RMS-normed and rotated; frequencies from rope_freqs, copied to the device.
+    void cache_append(const float* x, uint32_t ld, uint32_t q_col0, uint32_t q_stride, uint32_t k_col0, uint32_t v_col0,
+                      uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len, const int32_t* pos,
+                      uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq,
+                      float amplitude, const float* wq, const float* wk, float eps, void* q, void* k, void* v,
+                      uint32_t k_stride)
+    {
+        check(mako_cache_append(ctx_, stream_, dtype_, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new, kv_len,
+                                pos, heads, kv_heads, dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v, k_stride));
+    }
+    // Drafted tokens over the cache and one another (mask null: a chain).
+    void attention_tree(const void* q, const void* k, const void* v, float* o, uint32_t batch, uint32_t n_tok,
+                        const int32_t* n_new, const int32_t* kv_len, uint32_t max_kv_len, uint32_t heads,
+                        uint32_t kv_heads, uint32_t dim, uint32_t k_stride, const uint32_t* mask = nullptr)
+    {
+        check(mako_attention_tree(ctx_, stream_, dtype_, q, k, v, o, batch, n_tok, n_new, kv_len, max_kv_len, heads,
+                                  kv_heads, dim, k_stride, mask));
+    }
+    // attention_decode that adds every key's attention weight to weight [batch][kv_heads][k_stride].
+    void attention_decode_weights(const void* q, const void* k, const void* v, float* o, float* weight, uint32_t batch,
+                                  const int32_t* kv_len, uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads,
+                                  uint32_t dim, uint32_t k_stride)
+    {
+        check(mako_attention_decode_weights(ctx_, stream_, dtype_, q, k, v, o, weight, batch, kv_len, max_kv_len, heads,
+                                            kv_heads, dim, k_stride));
+    }
+    // Each sequence cut to `budget` rows by weight, into another cache or (equal pointers) in place.
+    void cache_evict(const void* k, const void* v, const float* weight, uint32_t batch, const int32_t* kv_len,
+                     uint32_t max_kv_len, uint32_t kv_heads, uint32_t dim, uint32_t k_stride, uint32_t sinks,
+                     uint32_t recent, uint32_t budget, void* k_out, void* v_out, float* weight_out, uint32_t out_stride,
+                     int32_t* kept, int32_t* new_len)
+    {
+        check(mako_cache_evict(ctx_, stream_, dtype_, k, v, weight, batch, kv_len, max_kv_len, kv_heads, dim, k_stride,
+                               sinks, recent, budget, k_out, v_out, weight_out, out_stride, kept, new_len));
+    }
     // The check gpu::Runtime::finish makes after a command buffer (src/gpu/runtime.cpp:466-471): throws if a
     // pipelined kernel gave up on a wait.  Synchronises the device.
     void finish()
@@ -169,6 +205,15 @@ private:
     Attention& attn_;
     mako_attn_group* g_ = nullptr;
 };
+
+// Angular frequencies of rotary positions (host), for cache_append.
+inline std::vector<double> rope_freqs(uint32_t rot, double theta, int scaling = MAKO_ROPE_PLAIN, double factor = 1.0,
+                                      double context = 0.0, double low = 0.0, double high = 0.0)
+{
+    std::vector<double> f(rot / 2 ? rot / 2 : 1);
+    Attention::check(mako_rope_freqs(rot, theta, scaling, factor, context, low, high, f.data()));
+    return f;
+}
 
 // The cube layout of a video sequence for the sparse path (src/models/h3.cpp:510-546): host arrays to copy to the
 // device (map [q_pad], valid [k_pad], cnt [n_cubes]) and the sizes the sparse calls take.  Throws as the reference

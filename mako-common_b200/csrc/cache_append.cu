@@ -6,7 +6,9 @@
 // heads: thread i makes pair i's while the heads' loads are in flight.  The angle pos * freq is taken in turns in
 // double precision and reduced to [-1/2, 1/2] there -- in fp32 a position of 10^6 would leave 0.06 radians of error --
 // and only the reduced turn goes through fp32 sincospi.  A warp takes up to HPW heads at a time, all their loads in
-// flight together, lane l holding values 4 l .. 4 l + 3 of every 128.
+// flight together (8 of 128 values: 108 us for 2 x 8192 tokens of 32 / 8 heads, 0.85 of the copy rate; 4: 122, 2: 211),
+// lane l holding values 4 l .. 4 l + 3 of every 128, so that a half rotation's partner is the same value of another
+// lane (through shared memory, with its bank conflicts, the same took 182 us).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -69,6 +71,10 @@ __global__ void cache_append_kernel(const AppendParams p)
                     v[j][n * VB + 1] = w.y;
                     v[j][n * VB + VB - 2] = w.z;
                     v[j][n * VB + VB - 1] = w.w;
+                } else if (VB == 2 && p.vec4) {
+                    const float2 w = __ldcs(reinterpret_cast<const float2*>(s));
+                    v[j][n * VB] = w.x;
+                    v[j][n * VB + 1] = w.y;
                 } else {
 #pragma unroll
                     for (int e = 0; e < VB; ++e)

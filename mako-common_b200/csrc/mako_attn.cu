@@ -976,8 +976,11 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
     if (uint64_t(max_kv_len) + n_tok > k_stride)
         return fail(MAKO_EINVAL, "tree: max_kv_len %u and %u drafted beyond the cache's %u rows", max_kv_len, n_tok,
                     k_stride);
-    if (batch > 65535 || uint64_t(n_tok) * heads > 65535)
-        return fail(MAKO_EINVAL, "tree: %u sequences of %u tokens, %u heads", batch, n_tok, heads);
+    if (batch > 65535)
+        return fail(MAKO_EINVAL, "tree: %u sequences (at most 65535)", batch);
+    // a sequence's key tiles, counted for every kv head and row block, fit 32 bits
+    if (((uint64_t(max_kv_len) + n_tok) / 64 + 1) * kv_heads * (uint64_t(heads / kv_heads) * n_tok / 128 + 1) > 0x7FFFFFFFull)
+        return fail(MAKO_EINVAL, "tree: %u keys for %u tokens of %u heads", max_kv_len, n_tok, heads);
     if (batch == 0 || n_tok == 0)
         return MAKO_OK;
     if (!q || !k || !v || !o || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
@@ -1029,8 +1032,10 @@ int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, c
         return rc;
     if (max_kv_len > k_stride)
         return fail(MAKO_EINVAL, "decode_weights: max_kv_len %u beyond the cache's %u rows", max_kv_len, k_stride);
-    if (batch > 65535 || heads > 65535)
-        return fail(MAKO_EINVAL, "decode_weights: %u sequences, %u heads", batch, heads);
+    if (batch > 65535 || kv_heads > 65535)
+        return fail(MAKO_EINVAL, "decode_weights: %u sequences, %u kv heads", batch, kv_heads);
+    if ((uint64_t(max_kv_len) / 64 + 1) * kv_heads * (uint64_t(heads / kv_heads) / 128 + 1) > 0x7FFFFFFFull)
+        return fail(MAKO_EINVAL, "decode_weights: %u keys for %u heads", max_kv_len, heads);
     if (batch == 0)
         return MAKO_OK;
     if (!q || !k || !v || !o || !weight || !kv_len || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
