@@ -10,7 +10,8 @@
 //     on the device from kv_len (no host synchronisation).  A segment within one CTA is written at once, the pieces of a
 //     cut one go to scratch (at most two a CTA) and tree_combine_kernel merges them by log-sum-exp.
 //   - Warp 0 streams K and V tiles by TMA through one ring in the order of use; warp 1 issues the products; warps 2 and
-//     3 load the rows of q, the latter cleans the drafted values; warps 4-11 are two softmax warpgroups, a thread a row.
+//     3 load the rows of q (the first piece's, for which all wait, the softmax warps do), the latter cleans the drafted
+//     values; warps 4-11 are two softmax warpgroups, a thread a row.
 //   - Up to 128 rows: the two warpgroups take alternate key tiles of the same rows, each with its own S, maximum, sum and
 //     O, and merge at the end (a split within the CTA).  More rows (WIDE): each takes 128 rows of every tile.  256-wide
 //     heads: O alone takes half of TMEM, so one warpgroup runs with two S buffers of 64 keys.
@@ -76,7 +77,7 @@ struct __align__(64) TreeParams {
     const void* q;
     const void* v;
     void* o;
-    float* o_part;    // [2 * grid][ROWS][D]
+    float* o_part;    // [2 * grid][D / 4][ROWS][4], DEC [2 * grid][ROWS][D]
     float2* ml_part;  // [2 * grid][ROWS]: (max in log2 units, sum)
     const int32_t* kv_len;
     const int32_t* n_new;
@@ -124,7 +125,7 @@ __device__ __forceinline__ SeqUnits seq_units(const TreeParams& p, uint32_t b)
 }
 // Down to one tile a CTA: 8 drafted tokens over 512 keys of 8 kv heads (40 tiles) run in 11.0 us so, 13.5 with two or
 // more tiles a CTA, 15.7 with four.
-__device__ __forceinline__ uint64_t units_per_cta(const TreeParams& p, uint64_t total)
+__device__ __forceinline__ uint32_t units_per_cta(const TreeParams& p, uint32_t total)
 {
     return total ? (total + p.grid - 1) / p.grid : 1;
 }
@@ -225,6 +226,28 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u)
     return m;
 }
 
+// Thread i of n copies its share of a piece's first `rows` rows of q into shared memory and zeroes the rows up to `upto`.
+template <class C, int D>
+__device__ __forceinline__ void load_q(const TreeParams& p, const Piece& x, uint32_t sQ, uint32_t i, uint32_t n, uint32_t rows,
+                                       uint32_t upto)
+{
+    constexpr uint32_t CH = D / 8;  // 16-byte chunks a row
+    const uint32_t step = n / CH, c = i % CH;
+    uint32_t r = i / CH, g = (x.rblk * C::ROWS + r) % p.group;
+    const uint16_t* const q = static_cast<const uint16_t*>(p.q);
+    const uint16_t* src =
+        q + ((uint64_t(x.b) * p.n_tok + (x.rblk * C::ROWS + r) / p.group) * p.heads + x.kvh * p.group + g) * D + c * 8;
+    for (; r < upto; r += step) {
+        cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128), r < rows ? src : q, r < rows);
+        src += step * D;
+        for (g += step; g >= p.group; g -= p.group)
+            src += (p.heads - p.group) * D;  // the group's heads of the next token
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+}
+
 template <int D, bool BF, bool WIDE, bool DEC>
 __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel(const __grid_constant__ TreeParams p)
 {
@@ -242,6 +265,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
     auto p_full = [&](uint32_t x) { return sB + 256 + 8 * x; };
     auto pv_done = [&](uint32_t x) { return sB + 272 + 8 * x; };
     const uint32_t q_full = sB + 288, q_empty = sB + 296, mma_done = sB + 304;
+    const uint32_t q_first = sB + 312;  // the first piece's rows of q
     volatile uint32_t* const plan = reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 320);  // b, rem, left, tmem
     volatile uint32_t* const dead = plan + 4;  // a softmax warp gave up
     uint32_t* const bad = reinterpret_cast<uint32_t*>(smem + C::BAD);
@@ -261,6 +285,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             mbar_init(pv_done(x), 1);
         }
         mbar_init(q_full, 64);
+        mbar_init(q_first, 128 * C::STREAMS);
         mbar_init(q_empty, 1);
         mbar_init(mma_done, 1);
         *dead = 0;
@@ -272,20 +297,20 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
     }
     if (warp == 0) {
         // this CTA's part of the line: [u0, u1), then the sequence u0 lies in
-        uint64_t units = lane < p.batch ? seq_units<C>(p, lane).units(p) : 0, total = units;
+        uint32_t units = lane < p.batch ? seq_units<C>(p, lane).units(p) : 0, total = units;
         for (uint32_t i = lane + 32; i < p.batch; i += 32)
             total += seq_units<C>(p, i).units(p);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
             total += __shfl_xor_sync(0xffffffffu, total, o);
-        const uint64_t per = units_per_cta(p, total), u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
-        uint64_t at = 0;
+        const uint32_t per = units_per_cta(p, total), u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
+        uint32_t at = 0;
         uint32_t b = 0, rem = 0;
         for (uint32_t i0 = 0; u0 < u1; i0 += 32) {
-            uint64_t incl = units;
+            uint32_t incl = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o)
                     incl += y;
             }
@@ -293,7 +318,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             if (hit) {
                 const int l = __ffs(hit) - 1;
                 b = i0 + l;
-                rem = uint32_t(u0 - at - __shfl_sync(0xffffffffu, incl - units, l));
+                rem = u0 - at - __shfl_sync(0xffffffffu, incl - units, l);
                 break;
             }
             at += __shfl_sync(0xffffffffu, incl, 31);
@@ -302,7 +327,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
         if (lane == 0) {
             plan[0] = b;
             plan[1] = rem;
-            plan[2] = uint32_t(u1 - u0);
+            plan[2] = u1 - u0;
         }
     }
     fence_before();
@@ -408,7 +433,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 x.t0 = __shfl_sync(0xffffffffu, x.t0, 0);
                 x.cached = __shfl_sync(0xffffffffu, x.cached, 0);
                 x.drafted = __shfl_sync(0xffffffffu, x.drafted, 0);
-                if (!(ok = mbar_wait_warp(q_full, pieces & 1, WAIT_LIMIT)))
+                if (!(ok = pieces ? mbar_wait_warp(q_full, (pieces - 1) & 1, WAIT_LIMIT) : mbar_wait_warp(q_first, 0, WAIT_LIMIT)))
                     break;
                 ++pieces;
                 if (WIDE) {
@@ -496,31 +521,17 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             // ---------------- q loaders, the second also cleans the drafted values ----------------
             // Rows past the drafted ones are zero: nobody reads what S and O hold for them, but products of zeros draw less
             // power, which is what holds the clock down here.
-            constexpr uint32_t CH = D / 8, RPI = 2 * (32 / CH);  // 16-byte chunks a row, rows the warps load at once
             uint32_t pieces = 0, used = 0;  // used: parity of each slot's v_raw uses so far
-            uint32_t dirty = ROWS;          // rows from here on are zero
+            uint32_t dirty = 0;             // rows from here on are zero
             while (ok && next_piece<C>(p, w, x)) {
                 if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
                     break;
-                {
-                    const uint32_t rows = min(ROWS, x.rows - x.rblk * ROWS), c = lane % CH;
-                    uint32_t r = (warp - 2) * (RPI / 2) + lane / CH;
-                    uint32_t tok = (x.rblk * ROWS + r) / p.group, g = (x.rblk * ROWS + r) % p.group;
-                    const uint16_t* src = static_cast<const uint16_t*>(p.q) +
-                                          ((uint64_t(x.b) * p.n_tok + tok) * p.heads + x.kvh * p.group + g) * D + c * 8;
-                    for (; r < max(rows, dirty); r += RPI) {
-                        cp_async16(sQ + (r >> 7) * C::QTILE + (c >> 3) * C::QBOX + swz(r & 127, c & 7, 128),
-                                   r < rows ? src : static_cast<const uint16_t*>(p.q), r < rows);
-                        src += RPI * D;
-                        for (g += RPI; g >= p.group; g -= p.group)
-                            src += (p.heads - p.group) * D;  // the group's heads of the next token
-                    }
-                    dirty = rows;
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    fence_proxy_async_smem();
+                const uint32_t rows = min(ROWS, x.rows - x.rblk * ROWS);
+                if (pieces > 0) {  // the softmax warps load the first piece's
+                    load_q<C, D>(p, x, sQ, threadIdx.x - 64, 64, rows, max(rows, dirty));
                     mbar_arrive(q_full);
                 }
+                dirty = rows;
                 if (warp == 2) {
                     ++pieces;
                     continue;
@@ -575,6 +586,10 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
         // sc: parity of each s_full's phases; pieces ended with tiles of this stream; tiles of all pieces so far
         uint32_t pieces = 0, sc = 0, ends = 0, products = 0;
         while (ok && next_piece<C>(p, w, x)) {
+            if (pieces == 0) {
+                load_q<C, D>(p, x, sQ, threadIdx.x - 128, 128 * C::STREAMS, min(ROWS, x.rows - x.rblk * ROWS), ROWS);
+                mbar_arrive(q_first);
+            }
             const uint32_t live_rows = x.rows;
             const uint32_t rbase = x.rblk * ROWS + (WIDE ? y * 128 : 0), r = rbase + row;
             const bool live = r < live_rows, warp_live = rbase + ql < live_rows;
@@ -784,8 +799,17 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                                 }
                             }
                     }
-                    if (live)
+                    if (live && (DEC || x.whole)) {
                         out_store32(dst, doff + c * 32, o, inv, x.whole ? p.o_type : 0u);
+                    } else if (live) {
+                        // A part, four columns at a time with the rows side by side: a warp's store is 512 bytes in one run
+                        // instead of 32 sectors of as many lines (7700 -> 4300 cycles for 128 rows of 256).
+                        float4* const d = reinterpret_cast<float4*>(p.o_part) + (uint64_t(x.slot) * (D / 4) + c * 8) * ROWS + lrow;
+#pragma unroll
+                        for (int g = 0; g < 8; ++g)
+                            d[g * ROWS] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
+                                                      __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
+                    }
                 }
             }
             fence_before();
@@ -815,11 +839,11 @@ struct RowPieces {
 };
 // Warp-collective.
 template <class C>
-__device__ __forceinline__ void line_sums(const TreeParams& p, uint32_t b, uint64_t& before, uint64_t& total)
+__device__ __forceinline__ void line_sums(const TreeParams& p, uint32_t b, uint32_t& before, uint32_t& total)
 {
     before = total = 0;
     for (uint32_t k = threadIdx.x & 31; k < p.batch; k += 32) {
-        const uint64_t n = seq_units<C>(p, k).units(p);
+        const uint32_t n = seq_units<C>(p, k).units(p);
         total += n;
         before += k < b ? n : 0;
     }
@@ -830,12 +854,12 @@ __device__ __forceinline__ void line_sums(const TreeParams& p, uint32_t b, uint6
     }
 }
 template <class C>
-__device__ __forceinline__ RowPieces row_pieces(const SeqUnits& s, uint32_t kvh, uint32_t r, uint64_t before, uint64_t per)
+__device__ __forceinline__ RowPieces row_pieces(const SeqUnits& s, uint32_t kvh, uint32_t r, uint32_t before, uint32_t per)
 {
-    const uint64_t u0 = before + uint64_t(kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
+    const uint32_t u0 = before + (kvh * s.rb + r / C::ROWS) * s.tiles, u1 = u0 + s.tiles;
     RowPieces x;
-    x.c0 = uint32_t(u0 / per);
-    x.c1 = uint32_t((u1 - 1) / per);
+    x.c0 = u0 / per;
+    x.c1 = (u1 - 1) / per;
     x.slot0 = 2 * x.c0 + (u0 % per ? 1 : 0);
     x.lrow = r % C::ROWS;
     return x;
@@ -859,14 +883,14 @@ __device__ __forceinline__ float merge_ml(float2 ml, float& M, float& l, float& 
     l = l * f0 + ls;
     return f;
 }
-// Merges the pieces of one row into o (values at o0 on): WARPS warps of the CTA take every WARPS-th group of pieces and
+// Merges the pieces of one row into o (values at o0 on, DEC): the CTA's WARPS warps take every WARPS-th group of pieces and
 // meet in shared memory.  parts: WARPS * (D + 2) floats.
 template <int D, class C, uint32_t WARPS>
 __device__ __forceinline__ void combine_row(const TreeParams& p, const RowPieces& x, uint64_t o0, float* parts)
 {
     constexpr uint32_t V = D / 32;
-    const uint32_t lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
-    const uint32_t step = WARPS == 1 ? 32 : min(32u, (x.c1 - x.c0) / WARPS + 1);  // pieces a warp takes at once
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t step = min(32u, (x.c1 - x.c0) / WARPS + 1);  // pieces a warp takes at once
     float M = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (uint32_t e = 0; e < V; ++e)
@@ -891,60 +915,89 @@ __device__ __forceinline__ void combine_row(const TreeParams& p, const RowPieces
             }
         }
     }
-    if (WARPS > 1) {
-        float* const mine = parts + warp * (D + 2);
-        if (lane == 0) {
-            mine[D] = M;
-            mine[D + 1] = l;
-        }
-#pragma unroll
-        for (uint32_t e = 0; e < V; ++e)
-            mine[lane * V + e] = acc[e];
-        __syncthreads();
-        M = -INFINITY;
-#pragma unroll
-        for (uint32_t k = 0; k < WARPS; ++k)
-            M = fmaxf(M, parts[k * (D + 2) + D]);
-        for (uint32_t d = threadIdx.x; d < D; d += WARPS * 32) {
-            float o = 0.0f, sum = 0.0f;
-#pragma unroll
-            for (uint32_t k = 0; k < WARPS; ++k) {
-                const float* const z = parts + k * (D + 2);
-                const float f = z[D] == -INFINITY ? 0.0f : ex2(z[D] - M);
-                o = fmaf(z[d], f, o);
-                sum = fmaf(z[D + 1], f, sum);
-            }
-            out_store1(p.o, o0 + d, sum != 0.0f ? o / sum : 0.0f, p.o_type);
-        }
-        return;
+    float* const mine = parts + warp * (D + 2);
+    if (lane == 0) {
+        mine[D] = M;
+        mine[D + 1] = l;
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (uint32_t e = 0; e < V; e += 2)
-        out_store2(p.o, o0 + lane * V + e, acc[e] * inv, acc[e + 1] * inv, p.o_type);
+    for (uint32_t e = 0; e < V; ++e)
+        mine[lane * V + e] = acc[e];
+    __syncthreads();
+    M = -INFINITY;
+#pragma unroll
+    for (uint32_t k = 0; k < WARPS; ++k)
+        M = fmaxf(M, parts[k * (D + 2) + D]);
+    for (uint32_t d = threadIdx.x; d < D; d += WARPS * 32) {
+        float o = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < WARPS; ++k) {
+            const float* const z = parts + k * (D + 2);
+            const float f = z[D] == -INFINITY ? 0.0f : ex2(z[D] - M);
+            o = fmaf(z[d], f, o);
+            sum = fmaf(z[D + 1], f, sum);
+        }
+        out_store1(p.o, o0 + d, sum != 0.0f ? o / sum : 0.0f, p.o_type);
+    }
 }
 
-// A warp a row: merges the pieces of a segment that several CTAs worked on; rows of segments written whole have
-// nothing to do.  Which pieces there are follows from the lengths alone and is worked out before the wait for the main
-// kernel; the weights of 32 pieces are made at once, a lane a piece, and their rows' loads do not depend on one another.
+// Merges the pieces of segments that several CTAs worked on by log-sum-exp; rows of segments written whole have nothing to
+// do.  A CTA takes 32 rows of one segment and 32 columns, a lane a row and a warp four columns, as the parts lie.
+// Which pieces there are follows from the lengths alone and is worked out before the wait for the main kernel.
 constexpr uint32_t CMB_WARPS = 8;
 template <int D, bool WIDE>
-__global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p)
+__global__ void __launch_bounds__(CMB_WARPS * 32) tree_combine_kernel(const __grid_constant__ TreeParams p, uint32_t blocks)
 {
     using C = TreeCfg<D, WIDE, false>;
-    const uint32_t b = blockIdx.y, per_kv = p.group * p.n_tok, i = blockIdx.x * CMB_WARPS + (threadIdx.x >> 5);
-    uint64_t before, total;
+    const uint32_t b = blockIdx.y, kvh = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t r0 = blockIdx.x % blocks * 32, r = r0 + lane;
+    uint32_t before, total;
     line_sums<C>(p, b, before, total);
     const SeqUnits s = seq_units<C>(p, b);
-    const uint32_t kvh = i / per_kv, r = i % per_kv;
     RowPieces x{};
-    if (kvh < p.kv_heads && r < p.group * s.drafted)
-        x = row_pieces<C>(s, kvh, r, before, units_per_cta(p, total));
+    if (r0 < p.group * s.drafted)
+        x = row_pieces<C>(s, kvh, r0, before, units_per_cta(p, total));
     // Every CTA waits, with rows or without: what comes next in the stream waits for this kernel alone.
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    if (x.c0 == x.c1)
+    if (x.c0 == x.c1 || r >= p.group * s.drafted)
         return;
-    combine_row<D, C, 1>(p, x, ((uint64_t(b) * p.n_tok + r / p.group) * p.heads + kvh * p.group + r % p.group) * D, nullptr);
+    x.lrow += lane;
+    const uint32_t col = (blockIdx.z * CMB_WARPS + warp) * 4;
+    float M = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr uint32_t AT = 8;  // pieces whose loads are in flight together
+    for (uint32_t cb = x.c0; cb <= x.c1; cb += AT) {
+        float2 ml[AT];
+        float4 z[AT];
+#pragma unroll
+        for (uint32_t k = 0; k < AT; ++k)
+            if (cb + k <= x.c1) {
+                ml[k] = p.ml_part[x.at<C>(cb + k)];
+                z[k] = __ldcs(reinterpret_cast<const float4*>(p.o_part) +
+                              (uint64_t(cb + k == x.c0 ? x.slot0 : 2 * (cb + k)) * (D / 4) + col / 4) * C::ROWS + x.lrow);
+            } else {
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                z[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        float Mn = M;
+#pragma unroll
+        for (uint32_t k = 0; k < AT; ++k)
+            Mn = fmaxf(Mn, ml[k].x);
+        const float f0 = M == -INFINITY ? 0.0f : ex2(M - Mn);
+        M = Mn;
+        l *= f0;  // l is 0, or NaN and stays so, while there is no maximum
+        acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+        for (uint32_t k = 0; k < AT; ++k) {
+            const float f = ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - M);
+            l = fmaf(ml[k].y, f, l);
+            acc = make_float4(fmaf(z[k].x, f, acc.x), fmaf(z[k].y, f, acc.y), fmaf(z[k].z, f, acc.z), fmaf(z[k].w, f, acc.w));
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t o = ((uint64_t(b) * p.n_tok + r / p.group) * p.heads + kvh * p.group + r % p.group) * D + col;
+    out_store2(p.o, o, acc.x * inv, acc.y * inv, p.o_type);
+    out_store2(p.o, o + 2, acc.z * inv, acc.w * inv, p.o_type);
 }
 
 // The second half of the decode with weights, for one kv head of a sequence.  CTAs below n_weight take WKEYS keys each:
@@ -959,10 +1012,10 @@ __global__ void __launch_bounds__(WNT) weights_finish_kernel(const __grid_consta
     __shared__ float2 ml[WHEADS];  // (max, 1 / sum) of up to WHEADS heads at a time
     __shared__ float parts[WNT / 32 * (D + 2)];
     const uint32_t b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t before, total;
+    uint32_t before, total;
     line_sums<C>(p, b, before, total);
     const SeqUnits s = seq_units<C>(p, b);
-    const uint64_t per = units_per_cta(p, total);
+    const uint32_t per = units_per_cta(p, total);
     asm volatile("griddepcontrol.wait;\n" ::: "memory");  // every CTA, as above
     if (blockIdx.x >= n_weight) {
         const uint32_t r = blockIdx.x - n_weight;
@@ -1089,9 +1142,9 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool bf, int* err, cudaStream_t st)
         return launch_dependent<const TreeParams, uint32_t>(weights_finish_kernel<D>, dim3(nw + nc, p.kv_heads, p.batch),
                                                             WNT, st, p, nw);
     } else {
-        return launch_dependent<const TreeParams>(
-            tree_combine_kernel<D, WIDE>,
-            dim3((p.group * p.n_tok * p.kv_heads + CMB_WARPS - 1) / CMB_WARPS, p.batch), CMB_WARPS * 32, st, p);
+        const uint32_t blocks = (p.group * p.n_tok + 31) / 32;
+        return launch_dependent<const TreeParams, uint32_t>(tree_combine_kernel<D, WIDE>, dim3(blocks * p.kv_heads, p.batch, D / 4 / CMB_WARPS),
+                                                            CMB_WARPS * 32, st, p, blocks);
     }
 }
 

@@ -978,8 +978,9 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
                     k_stride);
     if (batch > 65535)
         return fail(MAKO_EINVAL, "tree: %u sequences (at most 65535)", batch);
-    // a sequence's key tiles, counted for every kv head and row block, fit 32 bits
-    if (((uint64_t(max_kv_len) + n_tok) / 64 + 1) * kv_heads * (uint64_t(heads / kv_heads) * n_tok / 128 + 1) > 0x7FFFFFFFull)
+    // the key tiles of all sequences, kv heads and row blocks are counted in 32 bits
+    if (double((uint64_t(max_kv_len) + n_tok) / 64 + 1) * batch * kv_heads * double(uint64_t(heads / kv_heads) * n_tok / 128 + 1) >
+        2147483647.0)
         return fail(MAKO_EINVAL, "tree: %u keys for %u tokens of %u heads", max_kv_len, n_tok, heads);
     if (batch == 0 || n_tok == 0)
         return MAKO_OK;
@@ -1034,7 +1035,7 @@ int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, c
         return fail(MAKO_EINVAL, "decode_weights: max_kv_len %u beyond the cache's %u rows", max_kv_len, k_stride);
     if (batch > 65535 || kv_heads > 65535)
         return fail(MAKO_EINVAL, "decode_weights: %u sequences, %u kv heads", batch, kv_heads);
-    if ((uint64_t(max_kv_len) / 64 + 1) * kv_heads * (uint64_t(heads / kv_heads) / 128 + 1) > 0x7FFFFFFFull)
+    if (double(max_kv_len / 64 + 1) * batch * kv_heads * double(heads / kv_heads / 128 + 1) > 2147483647.0)
         return fail(MAKO_EINVAL, "decode_weights: %u keys for %u heads", max_kv_len, heads);
     if (batch == 0)
         return MAKO_OK;
