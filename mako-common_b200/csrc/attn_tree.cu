@@ -37,9 +37,9 @@ namespace {
 using namespace tc;
 
 constexpr long long WAIT_LIMIT = 1ll << 31;  // clock cycles (~1 s)
-// Pieces whose bad-value words are kept apart: the cleaner is at most a ring of loads (10 tiles, 5 pieces of one tile)
-// ahead of the epilogue that reads them.
-constexpr uint32_t BAD_RING = 8;
+// Pieces whose bad-value words are kept apart: the cleaner begins a piece once the products of the one before have all been
+// issued, when the epilogue of the one three before it is over.
+constexpr uint32_t BAD_RING = 4;
 
 template <int D, bool WIDE, bool DEC>
 struct TreeCfg {
@@ -291,6 +291,8 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
         *dead = 0;
         fence_barrier_init();
     }
+    if (warp == 3 && lane < 8)
+        bad[lane] = 0;
     if (warp == 2) {
         tmem_alloc(base + C::MISC + 332, 512);
         tmem_relinquish();
@@ -527,19 +529,18 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 if (pieces > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (pieces - 1) & 1, WAIT_LIMIT))))
                     break;
                 const uint32_t rows = min(ROWS, x.rows - x.rblk * ROWS);
+                uint32_t* const mybad = bad + pieces % BAD_RING * 8;
                 if (pieces > 0) {  // the softmax warps load the first piece's
+                    if (warp == 3 && lane < 8)
+                        mybad[lane] = 0;  // before q_full, on which the piece's epilogue depends
                     load_q<C, D>(p, x, sQ, threadIdx.x - 64, 64, rows, max(rows, dirty));
+                    __syncwarp();
                     mbar_arrive(q_full);
                 }
                 dirty = rows;
-                if (warp == 2) {
-                    ++pieces;
+                ++pieces;
+                if (warp == 2)
                     continue;
-                }
-                uint32_t* const mybad = bad + pieces++ % BAD_RING * 8;
-                if (lane < 8)
-                    mybad[lane] = 0;
-                __syncwarp();
                 const uint32_t first = x.cached / TK;  // the first tile with keys past the cached ones
                 for (uint32_t t = first > x.t0 ? first - x.t0 : 0; t < x.nb; ++t) {
                     const uint32_t j0 = (x.t0 + t) * TK, s = (n0 + v_at<WIDE>(t, x.nb)) % NS;
