@@ -6,8 +6,11 @@ import torch
 
 DT = {0: torch.float16, 1: torch.bfloat16}
 HALF_STEP = {0: 2.0 ** -11, 1: 2.0 ** -8}  # of the 16-bit type, relative
-# P is rounded to fp16, or kept as a bf16 value and the bf16 of what that left over
-P_STEP = {0: 2.0 ** -11, 1: 2.0 ** -16}
+# P is rounded to fp16 (2^-11 of p at most), for bf16 caches too where there are many rows and 16 keys' largest value lies in
+# [2^-8, 2^16): those values then go through fp16, exact but below 2^-14, where they are off by at most 2^-25, under 2^-17
+# of that largest.  Else P is the bf16 of p and the bf16 of what that left over, 2^-16 of p.
+P_STEP = {0: 2.0 ** -11, 1: 2.0 ** -11}
+V_STEP = {0: 0.0, 1: 2.0 ** -25}
 
 
 def randn(seed, *shape, dtype=0):
@@ -47,7 +50,8 @@ def attend(q, k, v, see, dtype):
 
     A score sums dim products in fp32: it is off by at most dim * 2^-24 * sum |q k| / sqrt(dim), the row's largest of
     which is e; a weight e^s and the sum it is divided by are off by that relatively, plus 2^-21 for the exponential and
-    the division, plus keys * 2^-24 for the sum.  Then o is off by those and P's rounding, times sum_j p_j |v_j|."""
+    the division, plus keys * 2^-24 for the sum.  Then o is off by those and P's rounding, times sum_j p_j |v_j|, and by V's
+    own."""
     q, k, v = q.double(), k.double(), v.double()
     dim, keys = q.shape[1], max(k.shape[0], 1)
     scale = 1.0 / math.sqrt(dim)
@@ -58,4 +62,4 @@ def attend(q, k, v, see, dtype):
     p = torch.nan_to_num(torch.softmax(s, -1))
     e = ((q.abs() @ k.abs().T) * scale * see).amax(-1, keepdim=True) * dim * 2.0 ** -24
     rel = 2.0 * e + 2.0 ** -21 + keys * 2.0 ** -24
-    return p @ v, p, (rel + keys * 2.0 ** -24 + P_STEP[dtype]) * (p @ v.abs()), rel
+    return p @ v, p, (rel + keys * 2.0 ** -24 + P_STEP[dtype]) * (p @ v.abs()) + V_STEP[dtype], rel

@@ -174,7 +174,7 @@ def test_unseen_values_have_no_effect(ctx, dtype, dim, n_tok):
         assert torch.isnan(g[sees][:, :H // KV]).all()
 
 
-@pytest.mark.parametrize("dim,n_tok", [(64, 5), (128, 5), (128, 70), (256, 5)])
+@pytest.mark.parametrize("dim,n_tok", [(64, 5), (128, 5), (64, 70), (128, 70), (256, 5)])
 def test_value_ranges(ctx, dim, n_tok):
     """bf16 values far outside fp16's range and at its ends, alike in all keys and by groups of 16 keys, and zero."""
     import cache_cases as C
@@ -190,6 +190,8 @@ def test_value_ranges(ctx, dim, n_tok):
         o = torch.full((1, n_tok, H * dim), 3.0, device="cuda")
         ctx.attention_tree(q, k, v, o, 1, n_tok, None, C.i32([L]), L, H, KV, dim, L + n_tok, mask)
         want, tol = want_rows(q[0], k[0], v[0], L, n_tok, see[0], 1)
+        if not torch.is_tensor(scale) and scale < 2.0 ** -11:
+            tol = tol - C.V_STEP[1]  # such values never go through fp16
         assert ((o[0].double() - want).abs() <= tol).all(), scale
 
 
@@ -220,6 +222,28 @@ def test_large_scores(ctx, dtype):
     ctx.attention_tree(q, k, v, o, 1, n, None, C.i32([L]), L, H, KV, D, L + n, mask)
     want, tol = want_rows(q[0], k[0], v[0], L, n, see[0], dtype)
     assert ((o[0].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,n_tok", [(0, 5), (0, 70), (1, 5), (1, 70)])
+def test_many_small_weights(ctx, dtype, n_tok):
+    """One key of weight 1 beside 32768 of 2^-25.1, all of one CTA, and values of 1: o is 1.  The small ones are 2^-10.1 of
+    the sum together.  Each P is off by 2^-6 of itself at most; the product's fp32 sum, near 2^7 in steps of 2^-16, takes
+    them 16 at a time, near 2^-14, and loses a step at most, a quarter: less than 2^-12 in all."""
+    import cache_cases as C
+    import mako_attn
+    import torch
+    D, L = 128, 32769
+    q = torch.ones(1, n_tok, 1, D, dtype=C.DT[dtype], device="cuda")
+    k = torch.zeros(1, 1, L + n_tok, D, dtype=C.DT[dtype], device="cuda")
+    k[0, 0, 0] = 1.5390625
+    v = torch.ones_like(k)
+    o = torch.zeros(1, n_tok, D, device="cuda")
+    ctx.set_option(mako_attn.OPT_GRID_CTAS, 1)
+    try:
+        ctx.attention_tree(q, k, v, o, 1, n_tok, None, C.i32([L]), L, 1, 1, D, L + n_tok)
+    finally:
+        ctx.set_option(mako_attn.OPT_GRID_CTAS, 0)
+    assert ((o.double() - 1).abs() <= 2.0 ** -11).all()
 
 
 def test_chain_of_one_is_decode(ctx):
