@@ -7,9 +7,12 @@
 // once, so that rows of equal weights do not queue at one counter.  All counts are integers: the result does not depend on
 // the order of the adds.  Then every warp, which owns consecutive rows, writes its kept rows' indices from the count of
 // those before it, ties taken from the lowest row on.
-// Bound by issue: about 40 instructions a key, 17 us for 24576 keys a row (26 with two CTAs a row, per-key warp votes around
-// the histogram and a guard on every unrolled key); a cluster barrier costs about 1500 cycles, so rows that fit one CTA's
-// registers take one.
+// Rows that do not compete take the key of a NaN, 0, which is the last of all: how many have it decides nothing, so no pass
+// asks again which rows compete, and a pass over a key is a handful of instructions.  The loop ends as soon as a digit's
+// count fits what is left to choose.  64 rows of 16-32K keys: the last is done after 14 us (21 with a test of every key in
+// every pass, four barriers a pass and the bits turned at the end), of which 3 are the load, 1 the keys, 1.2 a pass over
+// them and 0.7 the search after it.  Two CTAs a row take as long (37.6 and 38.1 us for the whole call): rows that fit one
+// CTA's registers take one.
 // evict_copy_kernel and evict_in_place_kernel copy the kept rows.  In place, row i comes from row kept[i] >= i: a CTA owns a
 // 64-byte column slice of every row and walks the rows upwards in steps, reading a whole step before it writes it, so what
 // a later step reads (rows at or past its own first) has not been written yet.
@@ -46,14 +49,24 @@ __device__ __forceinline__ uint32_t warp_incl_scan(uint32_t x)
     return x;
 }
 
+// Bits k with lo <= first + k < hi.
+__device__ __forceinline__ uint32_t bits_within(uint32_t first, uint32_t lo, uint32_t hi)
+{
+    auto under = [&](uint32_t end) {  // bits k with first + k < end
+        return end <= first ? 0u : end - first >= 32 ? 0xFFFFFFFFu : (1u << (end - first)) - 1u;
+    };
+    return under(hi) & ~under(lo);
+}
+
 // REG: a thread's keys fit its SKEYS registers.  blockDim.x: 256 or 1024.
 template <bool REG>
 __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
 {
-    __shared__ uint32_t hist[SBINS], sum[SBINS], part[32], mine[2], ranks[2][32];
+    __shared__ uint32_t hist[3][SBINS], sum[SBINS], part[3][32], found[3][2], mine[2], ranks[2][32];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank(), nt = blockDim.x, warps = nt / 32;
     const uint32_t kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the copy's CTAs wait in place for the end
     const int32_t l = p.kv_len[b];
     const uint32_t len = l > 0 ? min(uint32_t(l), p.max_len) : 0u, keep = min(len, p.budget);
     const uint64_t row = uint64_t(b) * p.kv_heads + kvh;
@@ -70,137 +83,151 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
     const float* const w = p.weight + row * p.k_stride;
     const uint32_t lo = p.sinks, hi = len - p.recent;  // the rows that compete
     uint32_t want = p.budget - p.sinks - p.recent;     // how many of them stay
-    const bool contest = want > 0;
-    // warp g of the cluster owns rows [g * 32 * nk, (g + 1) * 32 * nk), lane i's every 32nd
-    const uint32_t nk = (len + C * nt - 1) / (C * nt), j0 = (rank * warps + warp) * 32 * nk + lane;
+    // warp g of the cluster owns rows [g * 32 * nk, (g + 1) * 32 * nk), lane i's every 32nd; in registers, fours of them
+    uint32_t nk = (len + C * nt - 1) / (C * nt);
+    if (REG)
+        nk = (nk + 3) & ~3u;
+    const uint32_t first = (rank * warps + warp) * 32 * nk, j0 = first + lane;
+    auto competes = [&](uint32_t j) { return j - lo < hi - lo; };  // lo <= j < hi
+    // A row that does not compete has key 0, as a NaN has.  Rows are counted from the highest key down and key 0 is the
+    // last, so how many have it never matters.
+    auto load = [&](uint32_t j) { return competes(j) ? __ldg(w + j) : __uint_as_float(0x7FC00000u); };
     uint32_t reg[REG ? SKEYS : 1];
     if (REG) {
 #pragma unroll
-        for (uint32_t i = 0; i < SKEYS; ++i) {
+        for (uint32_t i = 0; i < SKEYS; i += 4) {
             if (i >= nk)
                 break;
-            reg[i] = j0 + i * 32 < len ? __float_as_uint(__ldg(w + j0 + i * 32)) : 0u;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                reg[REG ? i + e : 0] = __float_as_uint(load(j0 + (i + e) * 32));
         }
     }
-    // f(row, key) over this thread's rows, the whole warp in step
+    for (uint32_t i = tid; i < 3 * SBINS; i += nt)
+        hist[i / SBINS][i % SBINS] = 0;
+    // f(i, key) over this thread's rows j0 + 32 i, the whole warp in step
     auto each = [&](auto f) {
         if (REG) {
 #pragma unroll
-            for (uint32_t i = 0; i < SKEYS; ++i) {
+            for (uint32_t i = 0; i < SKEYS; i += 4) {
                 if (i >= nk)
                     break;
-                f(j0 + i * 32, reg[REG ? i : 0]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    f(i + e, reg[REG ? i + e : 0]);
             }
         } else {
             for (uint32_t i = 0; i < nk; ++i) {
-                uint32_t key = j0 + i * 32 < len ? weight_key(__ldg(w + j0 + i * 32)) : 0u;
-                f(j0 + i * 32, key);
+                uint32_t key = weight_key(load(j0 + i * 32));
+                f(i, key);
             }
         }
     };
-    auto competes = [&](uint32_t j) { return j - lo < hi - lo; };  // lo <= j < hi
-    // REG: the rows that compete, and those kept in any case, as bits of this thread's keys.  The bits in which the
-    // warp's competing keys differ from one another, and all that any of them has.
-    uint32_t comp = 0, sure_bits = 0, ones = 0, zeros = 0, counted = 0, bit = 1;
-    each([&](uint32_t j, uint32_t& key) {
-        const bool c = competes(j);
-        if (REG) {
+    // The bits in which the warp's keys differ from one another, and all that any of them has.
+    uint32_t ones = 0, all_ones = 0xFFFFFFFFu;
+    each([&](uint32_t, uint32_t& key) {
+        if (REG)
             key = weight_key(__uint_as_float(key));
-            comp |= c ? bit : 0u;
-            sure_bits |= !c && j < len ? bit : 0u;
-            bit <<= 1;
-        } else {
-            counted += c ? 1u : 0u;
-        }
-        ones |= c ? key : 0u;
-        zeros |= c ? ~key : 0u;
+        ones |= key;
+        all_ones &= key;
     });
-    if (REG)
-        counted = __popc(comp);
     ones = __reduce_or_sync(0xffffffffu, ones);
-    const uint32_t differ = ones & __reduce_or_sync(0xffffffffu, zeros), warp_counted = __reduce_add_sync(0xffffffffu, counted);
-    // T: the key of the last that stays, digit by digit; want: how many with key T stay
-    uint32_t T = 0;
-    for (uint32_t pass = 0; contest && pass < 3; ++pass) {
+    const uint32_t differ = ones & ~__reduce_and_sync(0xffffffffu, all_ones);
+    __syncthreads();
+    // T: the key of the last that stays, digit by digit; want: how many with key T stay.  No contest: no key is above T.
+    uint32_t T = want > 0 ? 0u : 0xFFFFFFFFu;
+    for (uint32_t pass = 0; want > 0 && pass < 3; ++pass) {
         const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
         const uint32_t fixed = pass == 0 ? 0u : 0xFFFFFFFFu << (pass == 1 ? 21 : 10);  // the digits that are known
-        for (uint32_t i = tid; i < bins; i += nt)
-            hist[i] = 0;
-        __syncthreads();
+        uint32_t* const h = hist[pass];
         if ((differ >> shift) == 0) {  // one digit, and one answer whether it counts, for the whole warp
-            if (lane == 0 && warp_counted && ((ones ^ T) & fixed) == 0)
-                atomicAdd(&hist[ones >> shift & (bins - 1)], warp_counted);
+            if (lane == 0 && ones && ((ones ^ T) & fixed) == 0)
+                atomicAdd(&h[ones >> shift & (bins - 1)], 32 * nk);
+        } else if (pass == 0) {
+            each([&](uint32_t, uint32_t& key) {
+                if (key)
+                    atomicAdd(&h[key >> 21], 1u);
+            });
         } else {
-            uint32_t m = comp;
-            each([&](uint32_t j, uint32_t& key) {
-                if ((REG ? (m & 1u) != 0 : competes(j)) && ((key ^ T) & fixed) == 0)
-                    atomicAdd(&hist[key >> shift & (bins - 1)], 1u);
-                m >>= 1;
+            each([&](uint32_t, uint32_t& key) {
+                if (((key ^ T) & fixed) == 0)
+                    atomicAdd(&h[key >> shift & (bins - 1)], 1u);
             });
         }
-        const uint32_t* all = hist;
+        const uint32_t* all = h;
         if (C > 1) {
             cluster.sync();
             for (uint32_t i = tid; i < bins; i += nt) {
                 uint32_t n = 0;
                 for (uint32_t c = 0; c < C; ++c)
-                    n += cluster.map_shared_rank(hist, c)[i];
+                    n += cluster.map_shared_rank(h, c)[i];
                 sum[i] = n;
             }
-            cluster.sync();  // no histogram is cleared before all have read it
             all = sum;
-        } else {
-            __syncthreads();
         }
+        __syncthreads();
         // The digit at which the count from the top reaches want: 32 groups of bins are summed a warp a group (or
-        // several), then every warp finds the group and the digit in it for itself.
+        // several), then one warp finds the group and the digit in it.
         const uint32_t per = bins / 32;  // 64 or 32 bins a group, group 0 the highest
         for (uint32_t g = warp; g < 32; g += warps) {
             const uint32_t top = bins - 1 - g * per - lane;
             const uint32_t n = __reduce_add_sync(0xffffffffu, all[top] + (per == 64 ? all[top - 32] : 0u));
             if (lane == 0)
-                part[g] = n;
+                part[pass][g] = n;
         }
         __syncthreads();
-        uint32_t n = part[lane], above = warp_incl_scan(n) - n;
-        const int g = 31 - __clz(__ballot_sync(0xffffffffu, above < want));  // the last group not past it
-        above = __shfl_sync(0xffffffffu, above, g);
-        uint32_t bin = bins - 1 - g * per - lane;
-        n = all[bin];
-        uint32_t before = above + warp_incl_scan(n) - n;
-        uint32_t last = __shfl_sync(0xffffffffu, before + n, 31);
-        if (per == 64 && last < want) {
-            bin -= 32;
+        if (warp == 0) {
+            uint32_t n = part[pass][lane], above = warp_incl_scan(n) - n;
+            const int g = 31 - __clz(__ballot_sync(0xffffffffu, above < want));  // the last group not past it
+            above = __shfl_sync(0xffffffffu, above, g);
+            uint32_t bin = bins - 1 - g * per - lane;
             n = all[bin];
-            before = last + warp_incl_scan(n) - n;
-        }
-        const int d = 31 - __clz(__ballot_sync(0xffffffffu, before < want));
-        T |= __shfl_sync(0xffffffffu, bin, d) << shift;
-        want -= __shfl_sync(0xffffffffu, before, d);
-        __syncthreads();  // hist and part are written again
-    }
-    // kept rows without the ties, and ties, of this warp; then of those before it
-    auto sure = [&](uint32_t j, uint32_t key) { return j < len && (!competes(j) || (contest && key > T)); };
-    auto tie = [&](uint32_t j, uint32_t key) { return contest && competes(j) && key == T; };
-    uint32_t n_sure = 0, n_tie = 0, tie_bits = 0;
-    if (contest || !REG) {
-        uint32_t m = comp;
-        bit = 1;
-        each([&](uint32_t j, uint32_t& key) {
-            if (REG) {
-                sure_bits |= (m & 1u) && key > T ? bit : 0u;
-                tie_bits |= (m & 1u) && key == T ? bit : 0u;
-                m >>= 1;
-                bit <<= 1;
-            } else {
-                n_sure += sure(j, key) ? 1u : 0u;
-                n_tie += tie(j, key) ? 1u : 0u;
+            uint32_t before = above + warp_incl_scan(n) - n;
+            const uint32_t last = __shfl_sync(0xffffffffu, before + n, 31);
+            if (per == 64 && last < want) {
+                bin -= 32;
+                n = all[bin];
+                before = last + warp_incl_scan(n) - n;
             }
-        });
+            if (int(lane) == 31 - __clz(__ballot_sync(0xffffffffu, before < want))) {
+                uint32_t t = T | bin << shift, left = want - before;
+                if (t && n == left) {  // all with these digits stay, whatever the others are
+                    t -= 1;
+                    left = 0;
+                }
+                found[pass][0] = t;
+                found[pass][1] = left;
+            }
+        }
+        __syncthreads();
+        T = found[pass][0];
+        want = found[pass][1];
     }
+    // Lane i takes the 32 rows of the warp's i-th keys from here on.  stay: those kept without the ties, tied: the ties
+    const uint32_t mine0 = first + lane * 32;
+    const uint32_t comp = lane < nk ? bits_within(mine0, lo, hi) : 0u, valid = lane < nk ? bits_within(mine0, 0, len) : 0u;
+    uint32_t stay = 0, tied = 0, n_sure = 0, n_tie = 0;
     if (REG) {
-        n_sure = __popc(sure_bits);
-        n_tie = __popc(tie_bits);
+        each([&](uint32_t i, uint32_t& key) {
+            const uint32_t a = __ballot_sync(0xffffffffu, key > T);
+            stay = lane == i ? a : stay;
+        });
+        stay |= valid & ~comp;
+        if (want > 0) {
+            each([&](uint32_t i, uint32_t& key) {
+                const uint32_t a = __ballot_sync(0xffffffffu, key == T);
+                tied = lane == i ? a : tied;
+            });
+            tied &= comp;
+        }
+        n_sure = __popc(stay);
+        n_tie = __popc(tied);
+    } else {
+        each([&](uint32_t i, uint32_t& key) {
+            const uint32_t j = j0 + i * 32;
+            n_sure += key > T || (j < len && !competes(j)) ? 1u : 0u;
+            n_tie += want > 0 && key == T && competes(j) ? 1u : 0u;
+        });
     }
     n_sure = __reduce_add_sync(0xffffffffu, n_sure);
     n_tie = __reduce_add_sync(0xffffffffu, n_tie);
@@ -229,40 +256,31 @@ __global__ void __launch_bounds__(SNT) evict_select_kernel(const EvictParams p)
         cluster.sync();  // no CTA leaves while others read its counts
     }
     at += min(ties, want);
-    const uint32_t below = (1u << lane) - 1u;
     if (n_sure == 0 && (n_tie == 0 || ties >= want))
         return;
     if (REG) {
-        // lane i takes the 32 rows of the warp's i-th keys
-        uint32_t stay = 0, tied = 0;
-        for (uint32_t i = 0; i < nk; ++i) {
-            const uint32_t a = __ballot_sync(0xffffffffu, sure_bits >> i & 1u);
-            stay = lane == i ? a : stay;
-        }
         if (n_tie) {  // the same for the warp
-            for (uint32_t i = 0; i < nk; ++i) {
-                const uint32_t a = __ballot_sync(0xffffffffu, tie_bits >> i & 1u);
-                tied = lane == i ? a : tied;
-            }
-            const uint32_t n = __popc(tied), first = ties + warp_incl_scan(n) - n;
-            for (uint32_t room = first < want ? want - first : 0u, k = n; k > room; --k)
+            const uint32_t n = __popc(tied), t0 = ties + warp_incl_scan(n) - n;
+            for (uint32_t room = t0 < want ? want - t0 : 0u, k = n; k > room; --k)
                 tied &= ~(0x80000000u >> __clz(tied));  // the highest go
             stay |= tied;
         }
         const uint32_t n = __popc(stay);
         at += warp_incl_scan(n) - n;
         for (; stay; stay &= stay - 1)
-            kept[at++] = int32_t(j0 - lane + lane * 32 + __ffs(stay) - 1);
+            kept[at++] = int32_t(mine0 + __ffs(stay) - 1);
     } else {
-        each([&](uint32_t j, uint32_t& key) {
-            const bool t = tie(j, key);
-            const uint32_t tied = __ballot_sync(0xffffffffu, t);
-            const bool stays = sure(j, key) || (t && ties + __popc(tied & below) < want);
-            const uint32_t stay = __ballot_sync(0xffffffffu, stays);
+        const uint32_t below = (1u << lane) - 1u;
+        each([&](uint32_t i, uint32_t& key) {
+            const uint32_t j = j0 + i * 32;
+            const bool t = key == T && competes(j);
+            const uint32_t ts = __ballot_sync(0xffffffffu, t);
+            const bool stays = key > T || (j < len && !competes(j)) || (t && ties + __popc(ts & below) < want);
+            const uint32_t st = __ballot_sync(0xffffffffu, stays);
             if (stays)
-                kept[at + __popc(stay & below)] = int32_t(j);
-            at += __popc(stay);
-            ties += __popc(tied);
+                kept[at + __popc(st & below)] = int32_t(j);
+            at += __popc(st);
+            ties += __popc(ts);
         });
     }
 }

@@ -182,6 +182,20 @@ def test_evict_long_rows(ctx, in_place):
     check_evict(ctx, 1, 1, 64, [300000], 0, 0, 290000, 300000, 300000, weight=np.float32(0.5), in_place=in_place)
 
 
+@pytest.mark.parametrize("n", [1500, 20000, 40001, 270001])
+@pytest.mark.parametrize("low,high", [(1.0, 2.0), (float(np.nextafter(np.float32(2), np.float32(0))), 2.0), (0.0, 1.0),
+                                      (float("nan"), 0.0), (1.0, float(np.nextafter(np.float32(1), np.float32(2)))),
+                                      (-float("inf"), -1.0)])
+def test_evict_counts_that_fit(ctx, n, low, high):
+    """Two weights, alike but for a digit or the last bit, of which just as many have the higher one as stay, or one more
+    or fewer; and no contest at all."""
+    rs = np.random.default_rng(n)
+    w = np.full(n, low)
+    w[7 + rs.permutation(n - 37)[:400]] = high
+    for budget in (437, 436, 438, 37):
+        check_evict(ctx, 0, 1, 64, [n], 7, 30, budget, n, budget, weight=w)
+
+
 def test_evict_capped_and_aliased_lengths(ctx):
     check_evict(ctx, 0, 2, 128, [900, 400, 1200], 4, 16, 256, 1300, 256, max_len=800)
     check_evict(ctx, 0, 4, 64, [900, 100, 1200], 4, 16, 256, 1300, 1300, in_place=True, alias_len=True)
