@@ -19,7 +19,8 @@
 //     2^-9; with few rows the tensor pipe has the room).  Base-2 softmax; a row's maximum moves only when passed by 8.
 //   - bf16 with many rows, where two products bound the time: each softmax warp turns 16 keys of the next V tile into fp16
 //     in shared memory while products run, and P is one fp16 part for them.  Keys whose largest |v| is not 0 and outside
-//     [2^-8, 2^16) stay bf16, with P in two parts; what fp16 rounds below 2^-14 is then under 2^-17 of that largest.
+//     [2^-8, 2^16) stay bf16, with P in two parts; what fp16 rounds below 2^-14 is then under 2^-17 of that largest.  So do
+//     16 keys with a drafted one among them: their values must not choose how rows that do not see it are rounded.
 //     64-token trees over 8 x 16-32K keys of 128: 253 -> 238 us at full clock, 295 -> 282 in a long run at the power cap.
 //   - Keys at or past the cached length are seen by mask.  Scores that are not seen are replaced, not added to, so keys may
 //     hold anything; values of those tiles are cleaned in shared memory before the product: rows behind the draft become
@@ -654,7 +655,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             }
             uint32_t top = __vmaxu2(__vmaxu2(best[0], best[1]), __vmaxu2(best[2], best[3]));
             top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-            const bool half = top == 0 || (top >= (119u << 7) && top < (143u << 7));  // 0, or [2^-8, 2^16)
+            // Cached keys alone, and 0 or in [2^-8, 2^16): a draft's value may not choose the rounding of rows that do not see it.
+            const bool half = (x.t0 + t) * TK + 16 * group + 16 <= x.cached &&
+                              (top == 0 || (top >= (119u << 7) && top < (143u << 7)));
             if (half) {
 #pragma unroll
                 for (uint32_t k = 0; k < NC; ++k)
