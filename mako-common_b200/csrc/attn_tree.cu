@@ -16,12 +16,11 @@
 //     O, and merge at the end (a split within the CTA).  More rows (WIDE): each takes 128 rows of every tile.  256-wide
 //     heads: O alone takes half of TMEM, so one warpgroup runs with two S buffers of 64 keys.
 //   - S is overwritten by P: fp16, or for bf16 the bf16 of p and of what that left over (two products, 2^-17 off instead of
-//     2^-9; with few rows the tensor pipe has the room).  Base-2 softmax; a row's maximum moves only when passed by 8.
-//   - bf16 with many rows, where two products bound the time: each softmax warp turns 16 keys of the next V tile into fp16
-//     in shared memory while products run, and P is one fp16 part for them.  Keys whose largest |v| is not 0 and outside
-//     [2^-8, 2^16) stay bf16, with P in two parts; what fp16 rounds below 2^-14 is then under 2^-17 of that largest.  So do
-//     16 keys with a drafted one among them: their values must not choose how rows that do not see it are rounded.
-//     64-token trees over 8 x 16-32K keys of 128: 253 -> 238 us at full clock, 295 -> 282 in a long run at the power cap.
+//     2^-9: the sum of many rounded weights would show in fp32 outputs).  Base-2 softmax; a row's maximum moves only when
+//     passed by 8.
+//   - Turning bf16 V tiles into fp16 in shared memory, so that P is one part, pays only if columns that are small beside the
+//     others may lose bits: with a test that fp16 holds every value exactly, 64-token trees over 8 x 16-32K keys take 248 us
+//     against 249 without, and without the test 237.
 //   - Keys at or past the cached length are seen by mask.  Scores that are not seen are replaced, not added to, so keys may
 //     hold anything; values of those tiles are cleaned in shared memory before the product: rows behind the draft become
 //     0, and so do single values that are not finite, which the rows that do see their token get back in the epilogue.
@@ -231,12 +230,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u)
     return m;
 }
 
-// Two bf16 values as fp16.
-__device__ __forceinline__ uint32_t bf_to_half2(uint32_t u)
-{
-    return Elem<__half>::pack(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
-}
-
 // Thread i of n copies its share of a piece's first `rows` rows of q into shared memory and zeroes the rows up to `upto`.
 template <class C, int D>
 __device__ __forceinline__ void load_q(const TreeParams& p, const Piece& x, uint32_t sQ, uint32_t i, uint32_t n, uint32_t rows,
@@ -279,13 +272,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
     const uint32_t q_first = sB + 312;  // the first piece's rows of q
     volatile uint32_t* const plan = reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 320);  // b, rem, left, tmem
     volatile uint32_t* const dead = plan + 4;  // a softmax warp gave up
-    // CONV: V tiles as fp16 where their values allow it
-    constexpr bool CONV = BF && WIDE;
-    auto v_ok = [&](uint32_t s) { return sB + 344 + 8 * s; };
     // P in fp16 is 2^RISE times the weight: at most 2^15 with the 2^8 by which a maximum may be passed, and that much further
     // from fp16's smallest values, where many small weights beside one large would be lost that the sum counts.
-    constexpr float RISE = BF && !WIDE ? 0.0f : 7.0f;
-    volatile uint8_t* const fmt = smem + C::MISC + 424;  // [NS][8] 16-key groups of the slot's V tile: 1 fp16, 0 bf16
+    constexpr float RISE = BF ? 0.0f : 7.0f;
     uint32_t* const bad = reinterpret_cast<uint32_t*>(smem + C::BAD);
     float2* const xchg = reinterpret_cast<float2*>(smem + C::XCHG);
 
@@ -296,8 +285,6 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
             mbar_init(v_raw(s), 1);
-            if (CONV)
-                mbar_init(v_ok(s), 256);
         }
         for (uint32_t x = 0; x < 2; ++x) {
             mbar_init(s_full(x), 1);
@@ -433,24 +420,6 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             auto pv = [&](uint32_t sbuf, uint32_t ot, uint32_t slot, uint32_t t, bool acc) {
                 const uint64_t b = dv + (slot * C::SLOT >> 4);
                 const uint32_t keys = x.cached + x.drafted - (x.t0 + t) * TK, d = tmem + COLO + ot * 128, a = tmem + sbuf * SC;
-                if constexpr (CONV) {
-                    constexpr uint32_t as_half = idesc_f16(0, 0, 0, 1, 128, D);
-                    volatile uint32_t* const f = reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 424 + slot * 8);
-                    const uint32_t f0 = __shfl_sync(0xffffffffu, f[0], 0), f1 = __shfl_sync(0xffffffffu, f[1], 0);
-                    if (keys >= TK && (f0 & f1) == 0x01010101u) {
-#pragma unroll
-                        for (uint32_t kk = 0; kk < TK / 16; ++kk)
-                            umma_ts_lead(lead, d, a + kk * 8, b + (kk * 2048 >> 4), as_half, acc || kk > 0);
-                    } else {
-                        for (uint32_t kk = 0; kk < (min(keys, TK) + 15) / 16; ++kk) {
-                            const bool half = (kk < 4 ? f0 >> (8 * kk) : f1 >> (8 * kk - 32)) & 1u;
-                            umma_ts_lead(lead, d, a + kk * 8, b + (kk * 2048 >> 4), half ? as_half : idesc_pv, acc || kk > 0);
-                            if (!half)
-                                umma_ts_lead(lead, d, a + TK / 2 + kk * 8, b + (kk * 2048 >> 4), idesc_pv, 1);
-                        }
-                    }
-                    return;
-                }
                 if (keys >= TK) {
 #pragma unroll
                     for (uint32_t part = 0; part < (BF ? 2 : 1); ++part)
@@ -465,7 +434,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                                     acc || part > 0 || kk > 0);
                 }
             };
-            uint32_t pieces = 0, pc = 0, vp = 0;  // pc, vp: parity of each p_full's and v_ok's phases so far
+            uint32_t pieces = 0, pc = 0;  // pc: parity of each p_full's phases so far
             auto wait_full = [&](uint32_t n) { return mbar_wait_warp(full(n % NS), (n / NS) & 1, WAIT_LIMIT); };
             auto wait_v = [&](uint32_t t) { return wait_full(n0 + v_at<WIDE>(t, x.nb)); };
             while (ok && next_piece<C>(p, w, x)) {
@@ -489,12 +458,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                         umma_commit_lead(lead, q_empty);
                     for (uint32_t t = 0; t < x.nb && ok; ++t) {
                         const uint32_t vs = (n0 + 2 * t + 1) % NS, ks = (n0 + 2 * t + 2) % NS;
-                        if (CONV) {
-                            ok = mbar_wait_warp(v_ok(vs), vp >> vs & 1u, WAIT_LIMIT);
-                            vp ^= 1u << vs;
-                        } else {
-                            ok = wait_v(t);
-                        }
+                        ok = wait_v(t);
                         for (uint32_t y = 0; y < 2 && ok; ++y) {
                             if (!(ok = mbar_wait_warp(p_full(y), pc >> y & 1u, WAIT_LIMIT)))
                                 break;
@@ -628,54 +592,12 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
         const uint32_t tl = tmem + (ql << 16);
         const float scale = p.scale_log2;
         // sc: parity of each s_full's phases; pieces ended with tiles of this stream; tiles of all pieces so far
-        uint32_t pieces = 0, sc = 0, ends = 0, products = 0, vp = 0;  // vp: parity of each v_ok's phases so far
-        // CONV: this warp's 16 keys of V tile t as fp16 where their largest value allows it, done while the products of
-        // the tile before run.
-        auto convert = [&](uint32_t t) {
-            constexpr uint32_t NC = D / 16;  // 16-byte chunks a lane
-            const uint32_t n = n0 + v_at<WIDE>(t, x.nb), slot = n % NS, group = 4 * y + (warp & 3);
-            if (!__all_sync(0xffffffffu, mbar_wait(full(slot), (n / NS) & 1, WAIT_LIMIT)))
-                return false;
-            uint8_t* const tile = smem + C::RING + slot * C::SLOT;
-            auto chunk = [&](uint32_t k) {
-                const uint32_t i = k * 32 + lane, rr = 16 * group + i / (D / 8), c = i % (D / 8);
-                return reinterpret_cast<uint4*>(tile + (c >> 3) * C::KBOX + swz(rr, c & 7, 128));
-            };
-            uint4 u[NC];
-            uint32_t best[4] = {0, 0, 0, 0};  // the largest magnitudes of the pairs' 16-bit halves
-#pragma unroll
-            for (uint32_t k = 0; k < NC; ++k)
-                u[k] = *chunk(k);
-#pragma unroll
-            for (uint32_t k = 0; k < NC; ++k) {
-                best[0] = __vmaxu2(best[0], u[k].x & 0x7FFF7FFFu);
-                best[1] = __vmaxu2(best[1], u[k].y & 0x7FFF7FFFu);
-                best[2] = __vmaxu2(best[2], u[k].z & 0x7FFF7FFFu);
-                best[3] = __vmaxu2(best[3], u[k].w & 0x7FFF7FFFu);
-            }
-            uint32_t top = __vmaxu2(__vmaxu2(best[0], best[1]), __vmaxu2(best[2], best[3]));
-            top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-            // Cached keys alone, and 0 or in [2^-8, 2^16): a draft's value may not choose the rounding of rows that do not see it.
-            const bool half = (x.t0 + t) * TK + 16 * group + 16 <= x.cached &&
-                              (top == 0 || (top >= (119u << 7) && top < (143u << 7)));
-            if (half) {
-#pragma unroll
-                for (uint32_t k = 0; k < NC; ++k)
-                    *chunk(k) = make_uint4(bf_to_half2(u[k].x), bf_to_half2(u[k].y), bf_to_half2(u[k].z), bf_to_half2(u[k].w));
-                fence_proxy_async_smem();
-            }
-            if (lane == 0)
-                fmt[slot * 8 + group] = half ? 1 : 0;
-            mbar_arrive(v_ok(slot));
-            return true;
-        };
+        uint32_t pieces = 0, sc = 0, ends = 0, products = 0;
         while (ok && next_piece<C>(p, w, x)) {
             if (pieces == 0) {
                 load_q<C, D>(p, x, sQ, threadIdx.x - 128, 128 * C::STREAMS, min(ROWS, x.rows - x.rblk * ROWS), ROWS);
                 mbar_arrive(q_first);
             }
-            if (CONV)
-                ok = convert(0);
             const uint32_t live_rows = x.rows;
             const uint32_t rbase = x.rblk * ROWS + (WIDE ? y * 128 : 0), r = rbase + row;
             const bool live = r < live_rows, warp_live = rbase + ql < live_rows;
@@ -683,7 +605,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
             float m = -INFINITY, l = 0.0f;
             uint32_t mine = 0;  // tiles of this stream so far
             const uint32_t step = WIDE || C::STREAMS == 1 ? 1 : 2;
-            for (uint32_t t = WIDE || C::STREAMS == 1 ? 0 : y; t < x.nb && ok; t += step, ++mine) {
+            for (uint32_t t = WIDE || C::STREAMS == 1 ? 0 : y; t < x.nb; t += step, ++mine) {
                 const uint32_t sb = WIDE ? y : t & 1;
                 ok = __all_sync(0xffffffffu, mbar_wait(s_full(sb), sc >> sb & 1u, WAIT_LIMIT));
                 if (!ok)
@@ -729,13 +651,6 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                     }
                     const float mneg = m == -INFINITY ? 0.0f : RISE - m;
                     const uint64_t scale2 = pack2(scale, scale), mneg2 = pack2(mneg, mneg);
-                    uint32_t vf[2] = {0, 0};  // CONV: which 16-key groups of V are fp16
-                    if (CONV) {
-                        const uint32_t vs = (n0 + v_at<WIDE>(t, x.nb)) % NS;
-                        ok = __all_sync(0xffffffffu, mbar_wait(v_ok(vs), vp >> vs & 1u, WAIT_LIMIT));
-                        vf[0] = *reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 424 + vs * 8);
-                        vf[1] = *reinterpret_cast<volatile uint32_t*>(smem + C::MISC + 428 + vs * 8);
-                    }
                     uint64_t sum2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
                     for (uint32_t c = 0; c < TK / 32; ++c) {
@@ -749,10 +664,7 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                             a = ex2(a);
                             b = ex2(b);
                             sum2[e & 1] = fadd2(sum2[e & 1], pack2(a, b));
-                            if (CONV) {
-                                hi[e] = __float_as_uint(a);
-                                lo[e] = __float_as_uint(b);
-                            } else if (BF) {
+                            if (BF) {
                                 hi[e] = Elem<__nv_bfloat16>::pack(a, b);
                                 lo[e] = Elem<__nv_bfloat16>::pack(a - __uint_as_float(hi[e] << 16),
                                                                   b - __uint_as_float(hi[e] & 0xFFFF0000u));
@@ -760,30 +672,8 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                                 hi[e] = Elem<__half>::pack(a, b);
                             }
                         }
-                        bool both = true;  // CONV: both of the chunk's 16-key groups of V are fp16
-                        if constexpr (CONV) {
-                            const uint32_t f = vf[c >> 1] >> ((c & 1) * 16);
-                            both = (f & 0x0101u) == 0x0101u;
-                            if (both) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    hi[e] = Elem<__half>::pack(__uint_as_float(hi[e]), __uint_as_float(lo[e]));
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const float a = __uint_as_float(hi[e]), b = __uint_as_float(lo[e]);
-                                    if (f >> (e / 8 * 8) & 1u) {
-                                        hi[e] = Elem<__half>::pack(a, b);
-                                    } else {
-                                        hi[e] = Elem<__nv_bfloat16>::pack(a, b);
-                                        lo[e] = Elem<__nv_bfloat16>::pack(a - __uint_as_float(hi[e] << 16),
-                                                                          b - __uint_as_float(hi[e] & 0xFFFF0000u));
-                                    }
-                                }
-                            }
-                        }
                         tmem_st16(tl + sb * SC + c * 16, hi);
-                        if (BF && !(CONV && both))
+                        if (BF)
                             tmem_st16(tl + sb * SC + TK / 2 + c * 16, lo);
                     }
                     {
@@ -815,11 +705,6 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 }
                 fence_before();
                 mbar_arrive(p_full(sb));
-                if (CONV) {
-                    vp ^= 1u << (n0 + v_at<WIDE>(t, x.nb)) % NS;
-                    if (ok && t + 1 < x.nb)
-                        ok = convert(t + 1);
-                }
                 if (!ok)
                     break;
                 if (DEC && live) {  // the row's scores, while the product runs; s_stride is a multiple of the tile
@@ -835,7 +720,6 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                         }
                 }
             }
-            n0 += 2 * x.nb;
             // The stream's last product.  One stream: on a barrier of its own, since pv_done(0) may by now have completed
             // one phase or two since S was seen, which a wait by parity cannot tell apart.
             if (ok && mine > 0) {

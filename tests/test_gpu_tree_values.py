@@ -1,9 +1,9 @@
 """What values do to mako_attention_tree and mako_attention_decode_weights in each of their layouts: up to 128 rows a kv
 head, more, and 256-wide heads.
 
-The bound on an output is that of cache_cases.attend with P's rounding as the layout has it.  bf16 caches of up to 128 rows
-or of 256-wide heads: P is the bf16 of p and the bf16 of what that left over, 2^-16 of p.  Else P is fp16, 2^-11 of p, and as
-it is held 2^7 up in steps of 2^-24 at least, 2^-32 of the largest weight where p is small.  V is exact everywhere."""
+The bound on an output is that of cache_cases.attend with P's rounding as the type has it.  bf16: P is the bf16 of p and the
+bf16 of what that left over, 2^-16 of p.  fp16: P is fp16, 2^-11 of p, and as it is held 2^7 up in steps of 2^-24 at least,
+2^-32 of the largest weight where p is small.  V is exact."""
 import numpy as np
 import pytest
 
@@ -16,17 +16,12 @@ BROAD = [(9, 8, 2, 256), (40, 8, 2, 256)]
 LAYOUTS = NARROW + WIDE + BROAD
 
 
-def two_parts(dtype, n_tok, group, dim):
-    return dtype == 1 and (dim == 256 or n_tok * group <= 128)
-
-
 def want_rows(q, k, v, cached, new, see, dtype):
     """o and its bound for one sequence: q [n][heads][dim], k, v [kv][S][dim], see [n][n]."""
     import cache_cases as C
     import torch
     n, H, D = q.shape
     G = H // k.shape[0]
-    two = two_parts(dtype, n, G, D)
     o = torch.zeros(n, H, D, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(o)
     vis = torch.cat([torch.ones(new, cached, dtype=torch.bool), torch.from_numpy(see[:new, :new])], 1).cuda()
@@ -34,8 +29,8 @@ def want_rows(q, k, v, cached, new, see, dtype):
         kk, vv = k[h // G, :cached + new], v[h // G, :cached + new]
         o[:new, h], p, _, rel = C.attend(q[:new, h], kk, vv, vis, dtype)
         size = vv.double().abs()
-        tol[:new, h] = (rel + (cached + new) * 2.0 ** -24 + (2.0 ** -16 if two else 2.0 ** -11)) * (p @ size)
-        if not two:
+        tol[:new, h] = (rel + (cached + new) * 2.0 ** -24 + (2.0 ** -16 if dtype else 2.0 ** -11)) * (p @ size)
+        if not dtype:
             tol[:new, h] += 2.0 ** -32 * (vis.double() @ size)
     return o, tol
 
@@ -92,3 +87,18 @@ def test_values_of_unseen_drafts(ctx, dtype, n_tok, heads, kv_heads, dim):
             blind = np.flatnonzero(~see[b, :new[b], j])
             assert blind.size
             assert (got[b, blind] == base[b, blind]).all(), (value, b)
+
+
+@pytest.mark.parametrize("n_tok,heads,kv_heads,dim", LAYOUTS)
+def test_small_columns(ctx, n_tok, heads, kv_heads, dim):
+    """bf16 value columns that are small beside the others, from ones that fp16 still holds to ones far below it: each is
+    as exact as the large ones.  First in all keys, then in every third group of sixteen."""
+    import torch
+    lens, new = [500, 33], [n_tok, n_tok - 2]
+    q, k, v0, see, mask = inputs(1, n_tok, heads, kv_heads, dim, lens)
+    scales = torch.tensor([1.0, 2.0 ** -12, 2.0 ** -16, 2.0 ** -18, 2.0 ** -20, 2.0 ** -26, 2.0 ** -60, 0.0],
+                          device="cuda").repeat(dim // 8)
+    group = torch.arange(v0.shape[2], device="cuda")[:, None] // 16
+    for scale in (scales, torch.where(group % 3 == 1, scales, 1.0)):
+        v = (v0.float() * scale).to(torch.bfloat16)
+        inside(call(ctx, q, k, v, lens, new, mask), q, k, v, lens, new, see, 1)
