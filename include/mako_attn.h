@@ -262,7 +262,9 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
  * floats (or 16-bit, MAKO_OPT_OUTPUT_16BIT), rows i >= n_new[b] left as they are, a row that sees nothing is 0.
  * A length above max_kv_len is read as max_kv_len; max_kv_len + n_tok is at most k_stride.  What cache rows hold that
  * no token of the sequence sees, NaN or infinities among it, has no effect, and neither has a drafted token on those
- * that do not see it.  Equal calls give equal results.  sm_100 only (MAKO_ENOTSUP otherwise). */
+ * that do not see it.  An infinite value that a row sees makes its column infinite with its sign, NaN where there are both
+ * signs or a NaN (weights that fp32 rounds to 0 aside).  Equal calls give equal results.  sm_100 only (MAKO_ENOTSUP
+ * otherwise). */
 int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
                         float* o, uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len,
                         uint32_t max_kv_len, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t k_stride,
@@ -270,7 +272,8 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
 
 /* mako_attention_decode that also accumulates every key's attention weight: weight [batch][kv_heads][k_stride] fp32
  * receives, at key j < kv_len[b], the sum over the kv head's query heads of softmax_j added to what it held; entries at
- * or past the length are left as they are.  The order of every sum is fixed: equal calls give equal results.
+ * or past the length are left as they are.  Infinite values count as in mako_attention_tree.  The order of every sum is
+ * fixed: equal calls give equal results.
  * batch and kv_heads at most 65535; sm_100 only (MAKO_ENOTSUP otherwise). */
 int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
                                   const void* v, float* o, float* weight, uint32_t batch, const int32_t* kv_len,

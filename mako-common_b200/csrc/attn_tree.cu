@@ -24,6 +24,7 @@
 //   - Keys at or past the cached length are seen by mask.  Scores that are not seen are replaced, not added to, so keys may
 //     hold anything; values of those tiles are cleaned in shared memory before the product: rows behind the draft become
 //     0, and so do single values that are not finite, which the rows that do see their token get back in the epilogue.
+//     Infinities among the cached values, seen by all, are looked for there once a row has NaN.
 //
 // The same kernel serves the decode that accumulates attention weights (DEC, mako_attention_decode_weights): one token a
 // sequence, its own key already counted in kv_len.  It stores the scores (4 bytes a key and head), and
@@ -228,6 +229,66 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u)
     if ((u >> 16 & e) == e)
         m |= 0xFFFF0000u;
     return m;
+}
+
+// Which of 32 columns of a row of values hold +inf, -inf, NaN: a bit each in r.x, r.y, r.z.
+template <bool BF>
+__device__ __forceinline__ void odd_columns(const uint16_t* row, uint3& r)
+{
+#pragma unroll 1
+    for (uint32_t e = 0; e < 32; e += 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row + e);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t h = w[i / 2] >> (i % 2 * 16), bit = 1u << (e + i);
+            if ((not_finite<BF>(h) & 0xFFFFu) == 0)
+                continue;
+            if (h & (BF ? 0x7Fu : 0x3FFu))
+                r.z |= bit;
+            else if (h & 0x8000u)
+                r.y |= bit;
+            else
+                r.x |= bit;
+        }
+    }
+}
+
+// The end of a piece some of whose values are not finite: in columns [c0, c1) (multiples of 32) every row (`on`) gets
+// what those it sees add up to, an infinity, or NaN where there are both or a NaN.  Drafted values are named by
+// the bits of bad; with `scan` the `keys` cached ones from key j0 on are read too.  Value d of this thread's row lies
+// at (d / 4) * step + d % 4 from `at`.  Warp-collective; out of line, so that it costs the others no registers.
+template <int D, bool BF>
+__device__ __noinline__ void odd_values(const TreeParams& p, uint32_t b, uint32_t kvh, uint32_t cached, uint32_t tok,
+                                        const uint32_t* bad, bool scan, uint32_t j0, uint32_t keys, uint32_t c0, uint32_t c1,
+                                        bool on, void* out, uint64_t at, uint32_t step, uint32_t type)
+{
+    const uint16_t* const v = static_cast<const uint16_t*>(p.v) + (uint64_t(b) * p.kv_heads + kvh) * p.k_hstride;
+#pragma unroll 1
+    for (uint32_t c = c0; c < c1; c += 32) {
+        uint3 r = make_uint3(0, 0, 0);
+        if (scan) {
+#pragma unroll 1
+            for (uint32_t j = threadIdx.x & 31; j < keys; j += 32)
+                odd_columns<BF>(v + uint64_t(j0 + j) * D + c, r);
+            r = make_uint3(__reduce_or_sync(0xffffffffu, r.x), __reduce_or_sync(0xffffffffu, r.y),
+                           __reduce_or_sync(0xffffffffu, r.z));
+        }
+        if (!on)
+            continue;
+#pragma unroll 1
+        for (uint32_t i = 0; i < 8; ++i)
+            for (uint32_t bits = bad[i]; bits; bits &= bits - 1) {
+                const uint32_t j = i * 32 + __ffs(bits) - 1;
+                if (token_sees(p, b, tok, j))
+                    odd_columns<BF>(v + uint64_t(cached + j) * D + c, r);
+            }
+        for (uint32_t bits = r.x | r.y | r.z; bits; bits &= bits - 1) {
+            const uint32_t e = __ffs(bits) - 1, d = c + e;
+            const float z = (r.z | (r.x & r.y)) >> e & 1u ? NAN : r.x >> e & 1u ? INFINITY : -INFINITY;
+            out_store1(out, at + uint64_t(d / 4) * step + d % 4, z, type);
+        }
+    }
 }
 
 // Thread i of n copies its share of a piece's first `rows` rows of q into shared memory and zeroes the rows up to `upto`.
@@ -764,8 +825,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 }
                 uint32_t any_bad = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < (DEC ? 0 : 8); ++i)
                     any_bad |= mybad[i];
+                bool nan = false;
                 // narrow: this warpgroup's half of the columns, of both parts
                 constexpr uint32_t NC = MERGE ? D / 64 : D / 32;
 #pragma unroll
@@ -790,24 +852,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                             o[e] = __float_as_uint(z);
                         }
                     }
-                    if (any_bad) {
-                        for (uint32_t i = 0; i < 8; ++i)
-                            for (uint32_t bits = mybad[i]; bits; bits &= bits - 1) {
-                                const uint32_t j = i * 32 + __ffs(bits) - 1;
-                                if (!token_sees(p, x.b, tok, j))
-                                    continue;
-                                const uint16_t* v = static_cast<const uint16_t*>(p.v) +
-                                                    (uint64_t(x.b) * p.kv_heads + x.kvh) * p.k_hstride +
-                                                    uint64_t(x.cached + j) * D + c * 32;
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const float u = BF ? __uint_as_float(uint32_t(v[e]) << 16)
-                                                       : __half2float(__ushort_as_half(v[e]));
-                                    if (!isfinite(u))
-                                        o[e] = __float_as_uint(__uint_as_float(o[e]) + u);
-                                }
-                            }
-                    }
+                    for (int e = 0; e < 32; ++e)
+                        nan |= isnan(__uint_as_float(o[e]));
                     if (live && (DEC || x.whole)) {
                         out_store32(dst, doff + c * 32, o, inv, x.whole ? p.o_type : 0u);
                     } else if (live) {
@@ -819,6 +866,16 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                             d[g * ROWS] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
                                                       __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
                     }
+                }
+                // A cached infinity gives NaN where its weight rounds to 0 in P, or to a second part of the other sign.  Scores
+                // of NaN make l NaN and the whole row.
+                const bool on = live && l > 0.0f, scan = __any_sync(0xffffffffu, nan && on);
+                if (scan || any_bad) {
+                    const bool rows = DEC || x.whole;
+                    const uint32_t c0 = MERGE ? y * (D / 2) : 0, j0 = x.t0 * TK, j1 = min(x.cached, j0 + x.nb * TK);
+                    odd_values<D, BF>(p, x.b, x.kvh, x.cached, tok, mybad, scan, j0, j1 > j0 ? j1 - j0 : 0u, c0,
+                                      c0 + NC * 32, on, dst, rows ? doff : (uint64_t(x.slot) * D * ROWS + lrow * 4),
+                                      rows ? 4u : 4 * ROWS, x.whole ? p.o_type : 0u);
                 }
             }
             fence_before();

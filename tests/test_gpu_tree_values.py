@@ -102,3 +102,90 @@ def test_small_columns(ctx, n_tok, heads, kv_heads, dim):
     for scale in (scales, torch.where(group % 3 == 1, scales, 1.0)):
         v = (v0.float() * scale).to(torch.bfloat16)
         inside(call(ctx, q, k, v, lens, new, mask), q, k, v, lens, new, see, 1)
+
+
+def spoil(v, lens, dim, kv=1):
+    """Non-finite values in cached rows: columns and what every row that sees them gets there.  Keys of several tiles, the
+    first and the last cached one among them."""
+    inf, nan = float("inf"), float("nan")
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        at = [0, n // 3, n // 2, n - 1]
+        v[b, kv, at[0], 2] = inf
+        v[b, kv, at[1], 5] = -inf
+        v[b, kv, at[2], 5] = -inf
+        v[b, kv, at[0], 9], v[b, kv, at[3], 9] = inf, -inf
+        v[b, kv, at[2], 33], v[b, kv, at[3], 33] = inf, nan
+        v[b, kv, at[3], dim - 1] = inf
+    return {2: inf, 5: -inf, 9: nan, 33: nan, dim - 1: inf}
+
+
+def same(a, value):
+    import torch
+    return (torch.isnan(a) if value != value else a == value).all()
+
+
+@pytest.mark.parametrize("ctas", [0, 2])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n_tok,heads,kv_heads,dim", LAYOUTS)
+def test_cached_infinities(ctx, dtype, n_tok, heads, kv_heads, dim, ctas):
+    """An infinite cached value makes its column infinite with its sign in every row of its kv head, whatever the weight it
+    has there; both signs, or NaN, make it NaN.  A drafted infinity of the other sign makes it NaN for those that see it."""
+    import torch
+    lens, new = [700, 0, 257], [n_tok, n_tok - 1, n_tok]
+    q, k, v, see, mask = inputs(dtype, n_tok, heads, kv_heads, dim, lens)
+    q = q * 6  # weights from 1 to far below fp16's smallest
+    G = heads // kv_heads
+    clean = v.clone()
+    columns = spoil(v, lens, dim)
+    o = call(ctx, q, k, v, lens, new, mask, ctas)
+    for b in (0, 2):
+        for d, value in columns.items():
+            assert same(o[b, :new[b], G:2 * G, d], value), (b, d)
+    rest = [d for d in range(dim) if d not in columns]
+    inside(o, q, k, clean, lens, new, see, dtype, rest)
+    for b in (0, 2):
+        v[b, 1, lens[b] + 1, 2] = float("-inf")
+        v[b, 1, lens[b] + 1, 5] = float("-inf")
+    o = call(ctx, q, k, v, lens, new, mask, ctas)
+    for b in (0, 2):
+        sees = torch.from_numpy(see[b, :new[b], 1]).cuda()
+        got = o[b, :new[b], G:2 * G]
+        assert same(got[sees][..., 2], float("nan")) and same(got[~sees][..., 2], float("inf"))
+        assert same(got[..., 5], float("-inf"))
+
+
+@pytest.mark.parametrize("ctas", [0, 2])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_cached_infinities_with_weights(ctx, dtype, dim, ctas):
+    """The same for the decode with weights, whose weights are those of finite values, bit for bit."""
+    import cache_cases as C
+    import mako_attn
+    import torch
+    lens, H, KV = [700, 0, 257, 1], 8, 2
+    q = C.randn(1, 4, H, dim, dtype=dtype) * 6
+    k, clean = C.randn(2, 4, KV, 700, dim, dtype=dtype), C.randn(3, 4, KV, 700, dim, dtype=dtype)
+    v = clean.clone()
+    columns = spoil(v, lens[:3], dim)
+
+    def decode(v):
+        o, w = torch.full((4, H * dim), 5.0, device="cuda"), torch.zeros(4, KV, 700, device="cuda")
+        ctx.set_option(mako_attn.OPT_GRID_CTAS, ctas)
+        try:
+            ctx.attention_decode_weights(q, k, v, o, w, C.i32(lens), 700, H, KV, dim, 700)
+        finally:
+            ctx.set_option(mako_attn.OPT_GRID_CTAS, 0)
+        torch.cuda.synchronize()
+        assert ctx.device_error() == 0
+        return o.view(4, H, dim), w
+
+    base, w0 = decode(clean)
+    o, w = decode(v)
+    assert torch.equal(w, w0)
+    rest = [d for d in range(dim) if d not in columns]
+    assert torch.equal(o[..., rest], base[..., rest]) and torch.equal(o[:, :4], base[:, :4])
+    for b in (0, 2):
+        for d, value in columns.items():
+            assert same(o[b, 4:, d], value), (b, d)
