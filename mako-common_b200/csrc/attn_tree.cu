@@ -800,7 +800,9 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 xchg[y * 128 + row] = make_float2(m, l);
                 if (!ok)
                     *dead = 1;
+                fence_before();  // either half reads both streams' O, of which it has waited for one
                 named_bar(1, 256);
+                fence_after();
                 ok = *dead == 0;  // a warp that gave up ends the walk of all, which meet at these barriers
                 const float2 a = xchg[row], b = xchg[128 + row];
                 const float M = fmaxf(a.x, b.x);
@@ -879,8 +881,10 @@ __global__ void __launch_bounds__((TreeCfg<D, WIDE, DEC>::NT), 1) tree_tc_kernel
                 }
             }
             fence_before();
-            if (MERGE)
+            if (MERGE) {
                 named_bar(1, 256);  // both have read both parts: the next piece's products may overwrite them
+                fence_after();
+            }
         }
         if (!ok && lane == 0)
             atomicExch(p.err, 44);

@@ -189,3 +189,20 @@ def test_cached_infinities_with_weights(ctx, dtype, dim, ctas):
     for b in (0, 2):
         for d, value in columns.items():
             assert same(o[b, 4:, d], value), (b, d)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_merged_streams_repeat(ctx, dtype, dim):
+    """Segments of one tile (whose second stream has none) to three, many a CTA: each of many calls gives the same bits,
+    within the bound."""
+    import torch
+    lens = [int(n) for n in np.random.default_rng(3).integers(0, 380, 60)]
+    new = [5] * 60
+    q, k, v, see, mask = inputs(dtype, 5, 8, 4, dim, lens)
+    base = call(ctx, q, k, v, lens, new, mask, 7)
+    inside(base, q, k, v, lens, new, see, dtype)
+    for ctas in (7, 3, 29, 0):
+        first = call(ctx, q, k, v, lens, new, mask, ctas)
+        for _ in range(10):
+            assert torch.equal(call(ctx, q, k, v, lens, new, mask, ctas), first)
