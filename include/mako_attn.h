@@ -218,8 +218,8 @@ int mako_proj(mako_attn_ctx* ctx, void* stream, int dtype, const void* w, const 
  * the one mako_attention_decode reads: k and v [batch][kv_heads][k_stride][dim] of `dtype`, kv_len [batch] int32 on the
  * device, dim 64, 128 or 256; an entry of kv_len <= 0 is an empty sequence.  A step of speculative decoding appends
  * the drafted tokens (mako_cache_append), attends them (mako_attention_tree) and raises kv_len by the accepted ones: of a
- * chain they lie in place, of a tree the caller appends them again, in order, behind kv_len.  A bounded cache decodes
- * with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls use is not
+ * chain they lie in place, of a tree the caller appends them again, in order, behind kv_len.  A bounded cache appends with
+ * mako_cache_append_weights, decodes with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls use is not
  * freed before the context is destroyed, so a CUDA graph that captured one stays valid when a later, larger call grows
  * it. */
 
@@ -255,6 +255,18 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
                       uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
                       const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride);
 
+/* mako_cache_append for a cache whose keys' attention weights are accumulated (mako_attention_decode_weights): sets
+ * weight [batch][kv_heads][k_stride] fp32 to 0 at every k / v row that it writes.  Decoding adds to what an entry holds and
+ * mako_cache_evict leaves the entries past the rows kept as they were, so without this a token would begin with the sum of
+ * the one whose row it takes over: after an eviction in place or into a cache that held more, or when a length is taken
+ * back.  weight null: mako_cache_append. */
+int mako_cache_append_weights(mako_attn_ctx* ctx, void* stream, int dtype, const float* x, uint32_t ld, uint32_t q_col0,
+                              uint32_t q_stride, uint32_t k_col0, uint32_t v_col0, uint32_t batch, uint32_t n_tok,
+                              const int32_t* n_new, const int32_t* kv_len, const int32_t* pos, uint32_t heads,
+                              uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq,
+                              float amplitude, const float* wq, const float* wk, float eps, void* q, void* k, void* v,
+                              uint32_t k_stride, float* weight);
+
 /* Attention for a tree of drafted tokens over a cache: q [batch][n_tok][heads][dim] (batch at most 65535, n_tok 256),
  * the drafted tokens' keys and values at cache rows kv_len[b] + i as mako_cache_append leaves them.  Token i < n_new[b]
  * (null: n_tok) sees the cached keys [0, kv_len[b]) and the drafted keys j < n_new[b] with bit j % 32 of
@@ -272,7 +284,8 @@ int mako_attention_tree(mako_attn_ctx* ctx, void* stream, int dtype, const void*
 
 /* mako_attention_decode that also accumulates every key's attention weight: weight [batch][kv_heads][k_stride] fp32
  * receives, at key j < kv_len[b], the sum over the kv head's query heads of softmax_j added to what it held; entries at
- * or past the length are left as they are.  Infinite values count as in mako_attention_tree.  The order of every sum is
+ * or past the length are left as they are, and have to be 0 once the length passes them (mako_cache_append_weights sees to
+ * it).  Infinite values count as in mako_attention_tree.  The order of every sum is
  * fixed: equal calls give equal results.
  * batch and kv_heads at most 65535; sm_100 only (MAKO_ENOTSUP otherwise). */
 int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
@@ -286,7 +299,7 @@ int mako_attention_decode_weights(mako_attn_ctx* ctx, void* stream, int dtype, c
  * their order, to rows 0, 1, ... of k_out and v_out [batch][kv_heads][out_stride][dim] and weight_out
  * [batch][kv_heads][out_stride]; kept [batch][kv_heads][budget] int32 receives the row each came from (-1 past their
  * number), new_len [batch] int32 min(kv_len, budget).  A sequence within the budget keeps all its rows.  Other rows of the
- * outputs are left as they are.  In place: k_out == k, v_out == v, weight_out == weight and out_stride == k_stride;
+ * outputs are left as they are, weight_out's too (mako_cache_append_weights clears them as they are written).  In place: k_out == k, v_out == v, weight_out == weight and out_stride == k_stride;
  * otherwise the outputs share no memory with the inputs (checked for equal addresses), except that new_len may be kv_len.
  * budget <= out_stride; a length above max_kv_len (<= k_stride) is read as max_kv_len; batch and kv_heads at most 65535. */
 int mako_cache_evict(mako_attn_ctx* ctx, void* stream, int dtype, const void* k, const void* v, const float* weight,

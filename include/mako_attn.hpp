@@ -98,14 +98,16 @@ public:
     }
     // ---- operators around a KV cache (no reference members): k, v [batch][kv_heads][k_stride][dim], kv_len [batch]
     // Projected tokens into the cache, q and k RMS-normed and rotated; frequencies from rope_freqs, copied to the device.
+    // weight [batch][kv_heads][k_stride], where attention weights are accumulated: 0 at the rows written.
     void cache_append(const float* x, uint32_t ld, uint32_t q_col0, uint32_t q_stride, uint32_t k_col0, uint32_t v_col0,
                       uint32_t batch, uint32_t n_tok, const int32_t* n_new, const int32_t* kv_len, const int32_t* pos,
                       uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq,
                       float amplitude, const float* wq, const float* wk, float eps, void* q, void* k, void* v,
-                      uint32_t k_stride)
+                      uint32_t k_stride, float* weight = nullptr)
     {
-        check(mako_cache_append(ctx_, stream_, dtype_, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new, kv_len,
-                                pos, heads, kv_heads, dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v, k_stride));
+        check(mako_cache_append_weights(ctx_, stream_, dtype_, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new,
+                                        kv_len, pos, heads, kv_heads, dim, rot, layout, freq, amplitude, wq, wk, eps, q, k,
+                                        v, k_stride, weight));
     }
     // Drafted tokens over the cache and one another (mask null: a chain).
     void attention_tree(const void* q, const void* k, const void* v, float* o, uint32_t batch, uint32_t n_tok,

@@ -197,6 +197,8 @@ __global__ void cache_append_kernel(const AppendParams p)
         }
         if (kind && row >= p.k_stride)
             continue;
+        if (kind == 1 && p.weight && lane < nh)  // a token begins without the weight of the one whose row it takes
+            p.weight[(uint64_t(b) * p.kv_heads + h0 + lane) * p.k_stride + row] = 0.0f;
         T* dst;
         uint64_t dstep;
         if (kind == 0) {

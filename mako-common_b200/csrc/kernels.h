@@ -133,6 +133,7 @@ struct AppendParams {
     void* q;  // [batch][n_tok][heads][dim]
     void* k;
     void* v;
+    float* weight;  // [batch][kv_heads][k_stride] or null: 0 at the rows written
     uint64_t ld;
     uint32_t q_col0, q_stride, k_col0, v_col0, batch, n_tok, heads, kv_heads, rot, layout, k_stride, vec4;
     float amplitude, eps;

@@ -909,6 +909,18 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
                       uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq, float amplitude,
                       const float* wq, const float* wk, float eps, void* q, void* k, void* v, uint32_t k_stride)
 {
+    return mako_cache_append_weights(ctx, stream, dtype, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new, kv_len,
+                                     pos, heads, kv_heads, dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v,
+                                     k_stride, nullptr);
+}
+
+int mako_cache_append_weights(mako_attn_ctx* ctx, void* stream, int dtype, const float* x, uint32_t ld, uint32_t q_col0,
+                              uint32_t q_stride, uint32_t k_col0, uint32_t v_col0, uint32_t batch, uint32_t n_tok,
+                              const int32_t* n_new, const int32_t* kv_len, const int32_t* pos, uint32_t heads,
+                              uint32_t kv_heads, uint32_t dim, uint32_t rot, int layout, const double* freq,
+                              float amplitude, const float* wq, const float* wk, float eps, void* q, void* k, void* v,
+                              uint32_t k_stride, float* weight)
+{
     if (int rc = cache_check(ctx, dtype, "cache_append", heads, kv_heads, dim))
         return rc;
     if (rot % 2 || rot > dim)
@@ -941,6 +953,7 @@ int mako_cache_append(mako_attn_ctx* ctx, void* stream, int dtype, const float* 
     p.q = q;
     p.k = k;
     p.v = v;
+    p.weight = weight;
     p.ld = ld;
     p.q_col0 = q_col0;
     p.q_stride = q_stride;

@@ -26,7 +26,7 @@ SYMBOLS = (
     "mako_peer_alloc", "mako_peer_free", "mako_peer_open", "mako_peer_close", "mako_group_create", "mako_group_connect",
     "mako_group_destroy", "mako_attention_gather", "mako_attention_decode_kv_sharded", "mako_group_connect_ptrs",
     "mako_group_area", "mako_heads", "mako_heads_norm", "mako_heads_partial", "mako_heads_clear",
-    "mako_cube_layout", "mako_proj", "mako_rope_freqs", "mako_cache_append",
+    "mako_cube_layout", "mako_proj", "mako_rope_freqs", "mako_cache_append", "mako_cache_append_weights",
     "mako_attention_tree", "mako_attention_decode_weights", "mako_cache_evict",
 )
 
@@ -87,6 +87,7 @@ def lib():
     L.mako_rope_freqs.argtypes = [u32, f64, i32, f64, f64, f64, f64, p]
     L.mako_cache_append.argtypes = ([p, p, i32, p] + [u32] * 7 + [p, p, p] + [u32] * 4 + [i32, p, f32, p, p, f32]
                                     + [p, p, p, u32])
+    L.mako_cache_append_weights.argtypes = L.mako_cache_append.argtypes + [p]
     L.mako_attention_tree.argtypes = [p, p, i32, p, p, p, p, u32, u32, p, p] + [u32] * 5 + [p]
     L.mako_attention_decode_weights.argtypes = [p, p, i32, p, p, p, p, p, u32, p] + [u32] * 5
     L.mako_cache_evict.argtypes = [p, p, i32, p, p, p, u32, p] + [u32] * 7 + [p, p, p, u32, p, p]
@@ -229,13 +230,15 @@ class Context:
 
     # -- operators around a KV cache k, v [batch][kv_heads][k_stride][dim], kv_len int32 [batch] (no reference counterpart)
     def cache_append(self, x, ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok, n_new, kv_len, pos, heads, kv_heads,
-                     dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v, k_stride, stream=None):
+                     dim, rot, layout, freq, amplitude, wq, wk, eps, q, k, v, k_stride, stream=None, weight=None):
         """mako_cache_append: x float32 rows -> q [batch][n_tok][heads][dim] and cache rows kv_len[b] + i, normed and
-        rotated; n_new, pos, wq, wk may be None, freq a float64 tensor [rot / 2] (None when rot is 0)."""
-        _check(lib().mako_cache_append(self._h, self._stream(stream), dtype_code(q), _ptr(x), ld, q_col0, q_stride,
-                                       k_col0, v_col0, batch, n_tok, _ptr(n_new), _ptr(kv_len), _ptr(pos), heads,
-                                       kv_heads, dim, rot, layout, _ptr(freq), amplitude, _ptr(wq), _ptr(wk), eps,
-                                       _ptr(q), _ptr(k), _ptr(v), k_stride))
+        rotated; n_new, pos, wq, wk may be None, freq a float64 tensor [rot / 2] (None when rot is 0).  weight float32
+        [batch][kv_heads][k_stride], where attention weights are accumulated: 0 at the rows written
+        (mako_cache_append_weights)."""
+        _check(lib().mako_cache_append_weights(self._h, self._stream(stream), dtype_code(q), _ptr(x), ld, q_col0, q_stride,
+                                               k_col0, v_col0, batch, n_tok, _ptr(n_new), _ptr(kv_len), _ptr(pos), heads,
+                                               kv_heads, dim, rot, layout, _ptr(freq), amplitude, _ptr(wq), _ptr(wk), eps,
+                                               _ptr(q), _ptr(k), _ptr(v), k_stride, _ptr(weight)))
 
     def attention_tree(self, q, k, v, o, batch, n_tok, n_new, kv_len, max_kv_len, heads, kv_heads, dim, k_stride,
                        mask=None, stream=None):
