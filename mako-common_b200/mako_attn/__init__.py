@@ -125,13 +125,36 @@ def _stream(stream):
     return ctypes.c_void_p(s.cuda_stream)
 
 
-def dtype_code(t) -> int:
+_CODES = {}  # torch dtype -> dtype code
+_F32 = _F64 = _I32 = _U32 = _raw_stream = None
+
+
+def _load_types():
+    """torch's types and stream query, looked up once: the calls on a cache are short."""
+    global _F32, _F64, _I32, _U32, _raw_stream
     import torch
-    if t.dtype == torch.float16:
-        return F16
-    if t.dtype == torch.bfloat16:
-        return BF16
-    raise TypeError(f"16-bit float tensors only, got {t.dtype}")
+    _F32, _F64, _I32, _U32 = torch.float32, torch.float64, torch.int32, torch.uint32
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    _CODES.update({torch.float16: F16, torch.bfloat16: BF16})
+
+
+def dtype_code(t) -> int:
+    if not _CODES:
+        _load_types()
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"16-bit float tensors only, got {t.dtype}")
+    return code
+
+
+def _typed(dtype, t):
+    """The address of a tensor, or None, of this dtype: the library would read another one past its end or as other
+    numbers."""
+    if t is None:
+        return None
+    if t.dtype is not dtype:
+        raise TypeError(f"{dtype} expected, got {t.dtype}")
+    return t.data_ptr()
 
 
 def attention_decode_noalloc(q, k, v, o, kv_len, max_kv_len, heads, kv_heads, dim, k_stride, stream=None):
@@ -158,6 +181,7 @@ def device_view(ptr: int, shape, typestr: str = "<i2"):
 
 class Context:
     """One mako_attn_ctx (its scratch and options) on a CUDA device."""
+    _out16 = False  # OPT_OUTPUT_16BIT
 
     def __init__(self, device: int = 0):
         self._h = ctypes.c_void_p()
@@ -177,6 +201,8 @@ class Context:
 
     def set_option(self, option: int, value: int):
         _check(lib().mako_attn_set_option(self._h, option, value))
+        if option == OPT_OUTPUT_16BIT:
+            self._out16 = bool(value)
 
     def device_error(self) -> int:
         """Reads and clears the device error flag (0: every pipelined wait completed)."""
@@ -235,38 +261,47 @@ class Context:
         rotated; n_new, pos, wq, wk may be None, freq a float64 tensor [rot / 2] (None when rot is 0).  weight float32
         [batch][kv_heads][k_stride], where attention weights are accumulated: 0 at the rows written
         (mako_cache_append_weights)."""
-        _check(lib().mako_cache_append_weights(self._h, self._stream(stream), dtype_code(q), _ptr(x), ld, q_col0, q_stride,
-                                               k_col0, v_col0, batch, n_tok, _ptr(n_new), _ptr(kv_len), _ptr(pos), heads,
-                                               kv_heads, dim, rot, layout, _ptr(freq), amplitude, _ptr(wq), _ptr(wk), eps,
-                                               _ptr(q), _ptr(k), _ptr(v), k_stride, _ptr(weight)))
+        code, t = dtype_code(q), q.dtype
+        if freq is not None and 2 * freq.numel() < rot <= dim:
+            raise ValueError(f"{freq.numel()} frequencies for {rot} rotated values")
+        _check(lib().mako_cache_append_weights(
+            self._h, self._stream(stream), code, _typed(_F32, x), ld, q_col0, q_stride, k_col0, v_col0, batch, n_tok,
+            _typed(_I32, n_new), _typed(_I32, kv_len), _typed(_I32, pos), heads, kv_heads, dim, rot, layout,
+            _typed(_F64, freq), amplitude, _typed(_F32, wq), _typed(_F32, wk), eps, q.data_ptr(), _typed(t, k), _typed(t, v),
+            k_stride, _typed(_F32, weight)))
 
     def attention_tree(self, q, k, v, o, batch, n_tok, n_new, kv_len, max_kv_len, heads, kv_heads, dim, k_stride,
                        mask=None, stream=None):
         """mako_attention_tree: q [batch][n_tok][heads][dim] over the cache and the n_new[b] (None: n_tok) drafted rows
         behind kv_len[b]; mask int32 or uint32 words [batch][n_tok][ceil(n_tok / 32)], None: a chain."""
-        _check(lib().mako_attention_tree(self._h, self._stream(stream), dtype_code(q), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
-                                         batch, n_tok, _ptr(n_new), _ptr(kv_len), max_kv_len, heads, kv_heads, dim,
-                                         k_stride, _ptr(mask)))
+        code, t = dtype_code(q), q.dtype
+        words = _I32 if mask is None or mask.dtype is _I32 else _U32
+        _check(lib().mako_attention_tree(
+            self._h, self._stream(stream), code, q.data_ptr(), _typed(t, k), _typed(t, v),
+            _typed(t if self._out16 else _F32, o), batch, n_tok, _typed(_I32, n_new), _typed(_I32, kv_len), max_kv_len,
+            heads, kv_heads, dim, k_stride, _typed(words, mask)))
 
     def attention_decode_weights(self, q, k, v, o, weight, kv_len, max_kv_len, heads, kv_heads, dim, k_stride,
                                  stream=None):
         """mako_attention_decode_weights: attention_decode that adds each key's weight to weight [batch][kv_heads][k_stride]."""
-        _check(lib().mako_attention_decode_weights(self._h, self._stream(stream), dtype_code(q), _ptr(q), _ptr(k), _ptr(v),
-                                                   _ptr(o), _ptr(weight), kv_len.numel(), _ptr(kv_len), max_kv_len,
-                                                   heads, kv_heads, dim, k_stride))
+        code, t = dtype_code(q), q.dtype
+        _check(lib().mako_attention_decode_weights(
+            self._h, self._stream(stream), code, q.data_ptr(), _typed(t, k), _typed(t, v),
+            _typed(t if self._out16 else _F32, o), _typed(_F32, weight), kv_len.numel(), _typed(_I32, kv_len), max_kv_len,
+            heads, kv_heads, dim, k_stride))
 
     def cache_evict(self, k, v, weight, kv_len, max_kv_len, kv_heads, dim, k_stride, sinks, recent, budget, k_out,
                     v_out, weight_out, out_stride, kept, new_len, stream=None):
         """mako_cache_evict: the kept rows of each sequence into k_out, v_out, weight_out (the inputs: in place)."""
-        _check(lib().mako_cache_evict(self._h, self._stream(stream), dtype_code(k), _ptr(k), _ptr(v), _ptr(weight),
-                                      kv_len.numel(), _ptr(kv_len), max_kv_len, kv_heads, dim, k_stride, sinks, recent,
-                                      budget, _ptr(k_out), _ptr(v_out), _ptr(weight_out), out_stride, _ptr(kept),
-                                      _ptr(new_len)))
+        code, t = dtype_code(k), k.dtype
+        _check(lib().mako_cache_evict(
+            self._h, self._stream(stream), code, k.data_ptr(), _typed(t, v), _typed(_F32, weight), kv_len.numel(),
+            _typed(_I32, kv_len), max_kv_len, kv_heads, dim, k_stride, sinks, recent, budget, _typed(t, k_out),
+            _typed(t, v_out), _typed(_F32, weight_out), out_stride, _typed(_I32, kept), _typed(_I32, new_len)))
 
     def _stream(self, stream):
-        """The stream given, or the current one of this context's device."""
-        import torch
-        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else stream.cuda_stream
+        """The stream given, or the current one of this context's device (after dtype_code)."""
+        return _raw_stream(self.device) if stream is None else stream.cuda_stream
 
     # -- TransformerRuntime::cube_select (src/models/runtime.cpp:286-303); returns (sel, nsel) as int16 tensor views
     # of the context's scratch ([heads][n_cubes][min(topk, n_cubes)] and [heads][n_cubes], uint16 bit patterns),
