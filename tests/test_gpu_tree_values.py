@@ -206,3 +206,117 @@ def test_merged_streams_repeat(ctx, dtype, dim):
         first = call(ctx, q, k, v, lens, new, mask, ctas)
         for _ in range(10):
             assert torch.equal(call(ctx, q, k, v, lens, new, mask, ctas), first)
+
+
+@pytest.mark.parametrize("ctas", [0, 1, 3])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n_tok,heads,kv_heads,dim", LAYOUTS)
+def test_values_that_are_not_finite(ctx, dtype, n_tok, heads, kv_heads, dim, ctas):
+    """NaN and infinities past the draft and in drafted values and keys: rows that do not see them keep their bits, rows
+    that do are infinite or NaN in those columns, or NaN whole for a key."""
+    import torch
+    lens, new, j, G = [190, 0, 700], [n_tok, n_tok - 1, n_tok], 1, heads // kv_heads
+    q, k, v, see, mask = inputs(dtype, n_tok, heads, kv_heads, dim, lens)
+    base = call(ctx, q, k, v, lens, new, mask, ctas)
+    inside(base, q, k, v, lens, new, see, dtype)
+    for b in range(3):
+        k[b, :, lens[b] + new[b]:] = float("nan")
+        v[b, :, lens[b] + new[b]:] = float("inf")
+    assert torch.equal(call(ctx, q, k, v, lens, new, mask, ctas), base)
+    k2, v2 = k.clone(), v.clone()
+    for b in range(3):
+        v2[b, 1, lens[b] + j, 3] = float("nan")
+        v2[b, 1, lens[b] + j, dim - 1] = float("-inf")
+        v2[b, 1, lens[b] + n_tok - 2, dim - 1] = float("inf")
+        k2[b, 0, lens[b] + j] = float("nan")
+    got = call(ctx, q, k, v2, lens, new, mask, ctas)
+    rest = [d for d in range(dim) if d not in (3, dim - 1)]
+    for b in range(3):
+        s, t = (torch.from_numpy(see[b, :new[b], x]).cuda() for x in (j, n_tok - 2))
+        g, w = got[b, :new[b]], base[b, :new[b]]
+        assert torch.equal(g[:, :G], w[:, :G]) and torch.equal(g[..., rest], w[..., rest])
+        assert torch.equal(g[~s][..., 3], w[~s][..., 3]) and torch.equal(g[~s & ~t], w[~s & ~t])
+        assert same(g[s][:, G:2 * G, 3], float("nan")) and same(g[s & ~t][:, G:2 * G, dim - 1], float("-inf"))
+        assert same(g[s & t][:, G:2 * G, dim - 1], float("nan")) and same(g[t & ~s][:, G:2 * G, dim - 1], float("inf"))
+    got = call(ctx, q, k2, v, lens, new, mask, ctas)
+    for b in range(3):
+        s = torch.from_numpy(see[b, :new[b], j]).cuda()
+        g, w = got[b, :new[b]], base[b, :new[b]]
+        assert torch.equal(g[~s], w[~s]) and torch.equal(g[:, G:], w[:, G:]) and same(g[s][:, :G], float("nan"))
+
+
+@pytest.mark.parametrize("ctas", [0, 1, 3])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n_tok,heads,kv_heads,dim", LAYOUTS)
+def test_maxima_that_move(ctx, dtype, n_tok, heads, kv_heads, dim, ctas):
+    """Scores that rise by more than 8 from tile to tile, for some rows and not for others, so that sums and outputs are
+    rescaled on the way; and scores in the thousands."""
+    import torch
+    lens, new = [900, 130], [n_tok, n_tok]
+    q, k, v, see, mask = inputs(dtype, n_tok, heads, kv_heads, dim, lens)
+    inside(call(ctx, q * 20, k * 10, v, lens, new, mask, ctas), q * 20, k * 10, v, lens, new, see, dtype)
+    # keys along one direction, growing with their row; every other token looks that way, the others away from it
+    along = (torch.arange(k.shape[2], device="cuda") / 100.0)[:, None].to(k.dtype)
+    k = (0.1 * k + along).contiguous()
+    sign = torch.tensor([1.0, -1.0], device="cuda").repeat(n_tok)[:n_tok, None, None].to(q.dtype)
+    q = (0.5 * q + sign).contiguous()
+    inside(call(ctx, q, k, v, lens, new, mask, ctas), q, k, v, lens, new, see, dtype)
+
+
+@pytest.mark.parametrize("exponent", [25.1, 20.5, 16.3])
+@pytest.mark.parametrize("dtype,n_tok,heads,dim", [(0, 5, 2, 128), (0, 70, 2, 128), (1, 5, 2, 128), (1, 70, 2, 128),
+                                                   (0, 70, 2, 64), (1, 70, 2, 64), (0, 5, 2, 256), (1, 70, 2, 256)])
+def test_many_small_weights(ctx, dtype, n_tok, heads, dim, exponent):
+    """One key of weight 1 beside 32768 of 2^-exponent, all of one CTA, and values of 1: o is 1.  The products are added to a
+    sum of 24 bits, which is never above o's own, and what lies below its last bit is cut off: 2^-23 of it a key at most,
+    2^-8 in all.  P's own error is 2^-11 of each of the small ones, 2^-6 for the first exponent, whose share of the sum
+    is below 2^-10: 2^-11 at most."""
+    import cache_cases as C
+    L = 32769
+    q = C.randn(1, 1, n_tok, heads, dim, dtype=dtype) * 0 + 1
+    k = C.randn(2, 1, 1, L + n_tok + 30, dim, dtype=dtype) * 0
+    k[0, 0, 0] = exponent * 0.6931471805599453 / dim ** 0.5
+    o = call(ctx, q, k, k * 0 + 1, [L], [n_tok], None, 1)
+    assert ((o.double() - 1).abs() <= 2.0 ** -8 + 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads,scale", [(8, 2, 1.0), (7, 1, 1.0), (40, 2, 1.0), (8, 8, 12.0)])
+def test_decode_with_weights_is_decode(ctx, dtype, dim, heads, kv_heads, scale):
+    """The decode with weights gives softmax's output within the bound of two-part weights for bf16, and what
+    attention_decode gives over the same cache, whose own error is bounded alike, within both bounds; the weights of a kv
+    head sum to its query heads."""
+    import cache_cases as C
+    import torch
+    lens, G = [1500, 0, 77, 1], heads // kv_heads
+    q = C.randn(1, 4, heads, dim, dtype=dtype) * scale
+    k, v = C.randn(2, 4, kv_heads, 1500, dim, dtype=dtype), C.randn(3, 4, kv_heads, 1500, dim, dtype=dtype)
+    a, d = (torch.full((4, heads * dim), 3.0, device="cuda") for _ in range(2))
+    w = torch.zeros(4, kv_heads, 1500, device="cuda")
+    ctx.attention_decode_weights(q, k, v, a, w, C.i32(lens), 1500, heads, kv_heads, dim, 1500)
+    ctx.attention_decode(q, k, v, d, C.i32(lens), 1500, heads, kv_heads, dim, 1500)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (a[b] == 0).all() and (d[b] == 0).all() and (w[b] == 0).all()
+            continue
+        want, tol = want_rows(q[b][None], k[b], v[b], n - 1, 1, np.ones((1, 1), bool), dtype)
+        x, y = (t[b].view(1, heads, dim).double() for t in (a, d))
+        assert ((x - want).abs() <= tol).all() and ((x - y).abs() <= 2 * tol).all()
+        # each weight within 2^-11 of itself for scores of tens in fp32 (dim * 2^-24 * 2 * sum |q k| / sqrt(dim))
+        assert ((w[b].double().sum(-1) - G).abs() <= G * 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n_tok,heads,kv_heads", [(1, 8, 8), (5, 8, 2), (33, 6, 2), (64, 8, 2), (129, 2, 1)])
+def test_two_part_weights(ctx, monkeypatch, dim, n_tok, heads, kv_heads):
+    """bf16 within the bound of P in two parts and exact values, at the sizes of the tests of shapes: one part would be
+    2^-9 off."""
+    import cache_cases as C
+    import test_gpu_cache_evict as E
+    import test_gpu_tree as T
+    monkeypatch.setattr(C, "P_STEP", {0: 2.0 ** -11, 1: 2.0 ** -16})
+    monkeypatch.setattr(C, "V_STEP", {0: 0.0, 1: 0.0})
+    T.run(ctx, 1, n_tok, heads, kv_heads, dim, [700, 0, 129], seed=n_tok + dim)
+    T.run(ctx, 1, n_tok, heads, kv_heads, dim, [0, 1500, 3, 200, 700], new=[n_tok, 5, 1, 0, n_tok], k_stride=1800, ctas=3)
+    E.check_weights(ctx, 1, heads, kv_heads, dim, [700, 0, 129, -4, 1, 3000], seed=heads + dim)
