@@ -48,14 +48,15 @@ enum {
      * multiple of 64 (raised when a sequence would need more than 1024 splits). */
     MAKO_OPT_DECODE_CHUNK = 3,
     /* 1: every call also records a CUDA event pair around its main kernel (the attention or split kernel, not the
-     * bf16 V pre-pass, the decode combine or the group barriers) for mako_attn_kernel_times; 0 (default): none. */
+     * bf16 V pre-pass, the decode combine or the group barriers; of the calls around a KV cache all kernels) for
+     * mako_attn_kernel_times; 0 (default): none. */
     MAKO_OPT_KERNEL_TIMING = 4,
-    /* 1: mako_attention, mako_attention_decode, mako_attention_sparse and mako_attention_block_sparse write o in the
-     * call's 16-bit type (the values the reference's to_half / to_bf16 pass makes of its fp32 o before the output
+    /* 1: mako_attention, mako_attention_decode, mako_attention_sparse, mako_attention_block_sparse, mako_attention_tree and
+     * mako_attention_decode_weights write o in the call's 16-bit type (the values the reference's to_half / to_bf16 pass makes of its fp32 o before the output
      * projection, src/gpu/runtime.cpp:164-190), 2 bytes per value, `o` pointing at that storage; o row widths of the
      * prefill paths a multiple of 8.  0 (default): fp32 o.  The sharded forms keep fp32 (MAKO_ENOTSUP when set). */
     MAKO_OPT_OUTPUT_16BIT = 5,
-    /* The persistent kernels' grid (tcgen05 dense and block-sparse attention, the output projection): 0 (default) one
+    /* The persistent kernels' grid (tcgen05 dense and block-sparse attention, trees, decode with weights, the output projection): 0 (default) one
      * CTA per SM; n > 0 at most n CTAs, each then working through more items -- for tests of the paths that carry
      * one item's state into the next on small problems. */
     MAKO_OPT_GRID_CTAS = 6
@@ -221,7 +222,8 @@ int mako_proj(mako_attn_ctx* ctx, void* stream, int dtype, const void* w, const 
  * chain they lie in place, of a tree the caller appends them again, in order, behind kv_len.  A bounded cache appends with
  * mako_cache_append_weights, decodes with mako_attention_decode_weights and now and then evicts (mako_cache_evict).  The scratch these calls use is not
  * freed before the context is destroyed, so a CUDA graph that captured one stays valid when a later, larger call grows
- * it. */
+ * it; graphs of one context share it and must not run at once.  The decode with weights takes batch * heads * max_kv_len
+ * floats of it. */
 
 /* Rotation partners: value i of the rotated part with i + rot / 2, or 2i with 2i + 1. */
 enum { MAKO_ROPE_HALVES = 1, MAKO_ROPE_PAIRS = 2 };
@@ -231,7 +233,8 @@ enum {
     MAKO_ROPE_LINEAR = 1, /* f_i / factor: positions interpolated */
     MAKO_ROPE_BASE = 2,   /* theta * factor^(rot / (rot - 2)): the slowest pair slowed by factor, the fastest kept */
     MAKO_ROPE_PARTS = 3   /* by parts: with r_i = context * f_i / (2 pi) turns over the trained context and
-                           * g_i = (r_i - low) / (high - low) clamped to [0, 1], f_i * (g_i + (1 - g_i) / factor) */
+                           * g_i = (r_i - low) / (high - low) clamped to [0, 1], f_i * (g_i + (1 - g_i) / factor);
+                           * models that ramp over i instead of r_i need a table of their own */
 };
 /* Host code, host array: the angular frequencies (radians a position) freq [rot / 2] of rotary positions with base
  * theta over the first rot values of a head.  factor (>= 1) is read by every scaling but MAKO_ROPE_PLAIN, context
@@ -272,7 +275,9 @@ int mako_cache_append_weights(mako_attn_ctx* ctx, void* stream, int dtype, const
  * (null: n_tok) sees the cached keys [0, kv_len[b]) and the drafted keys j < n_new[b] with bit j % 32 of
  * mask[b][i][j / 32] set (uint32 [batch][n_tok][(n_tok + 31) / 32]; null: j <= i, a chain); o [batch][n_tok][heads * dim]
  * floats (or 16-bit, MAKO_OPT_OUTPUT_16BIT), rows i >= n_new[b] left as they are, a row that sees nothing is 0.
- * A length above max_kv_len is read as max_kv_len; max_kv_len + n_tok is at most k_stride.  What cache rows hold that
+ * A length above max_kv_len is read as max_kv_len; max_kv_len + n_tok is at most k_stride.  Scores and sums are fp32; the
+ * softmax's weights multiply the values as fp16 (2^-11 of each) for fp16 caches, as two bf16 parts (2^-16) for bf16
+ * caches.  What cache rows hold that
  * no token of the sequence sees, NaN or infinities among it, has no effect, and neither has a drafted token on those
  * that do not see it.  An infinite value that a row sees makes its column infinite with its sign, NaN where there are both
  * signs or a NaN (weights that fp32 rounds to 0 aside).  Equal calls give equal results.  sm_100 only (MAKO_ENOTSUP
